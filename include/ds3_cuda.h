@@ -382,6 +382,93 @@ int ds3_cuda_moe_combine_residual(const ds3_cuda_buffer_t *y, const ds3_cuda_buf
                                   uint32_t n_tokens, uint32_t n_used, uint32_t n_cols);
 
 /* ------------------------------------------------------------------ */
+/* Microscaled (MX) rows and the experts' products over them (new)    */
+/* ------------------------------------------------------------------ */
+
+/* An MX row of n elements is n/32 blocks, each with one power-of-two scale
+ * byte: value = 2^(scale - 127) * element (OCP Microscaling Formats v1.0).
+ *  - DS3_CUDA_MXFP8: elements e4m3, n bytes per row;
+ *  - DS3_CUDA_MXFP4: elements e2m1, n/2 bytes per row, element 2i in the low
+ *    nibble of byte i.
+ * Elements and scales are separate dense buffers, [rows][n or n/2] and
+ * [rows][n/32] bytes. A block's scale comes from its largest magnitude's
+ * exponent; elements round to nearest even and saturate. A block that holds
+ * an infinity or NaN gets scale 255 (NaN) and zero elements, so that all of it
+ * reads as NaN. Element buffers must be 16-byte aligned (32 for MXFP4 weights
+ * of the products below). Outputs must not overlap inputs unless said so. */
+typedef enum { DS3_CUDA_MXFP8 = 0, DS3_CUDA_MXFP4 = 1 } ds3_cuda_mx_t;
+
+/* Rows of `src_type` (DS3_TYPE_F32 or DS3_TYPE_F16; dequantize_f32 first for
+ * other types) to MX rows. n_cols % 32 == 0; src 16-byte aligned. */
+int ds3_cuda_mx_quantize(const ds3_cuda_buffer_t *src, ds3_type_t src_type,
+                         ds3_cuda_buffer_t *q, ds3_cuda_buffer_t *scales, ds3_cuda_mx_t to,
+                         uint64_t n_rows, uint32_t n_cols);
+
+/* The fp32 values of MX rows (exact). dst 16-byte aligned. */
+int ds3_cuda_mx_dequantize(const ds3_cuda_buffer_t *q, const ds3_cuda_buffer_t *scales, ds3_cuda_mx_t from,
+                           ds3_cuda_buffer_t *dst, uint64_t n_rows, uint32_t n_cols);
+
+/* add_rms_norm with MXFP8 output: s = x + residual, norm = s / sqrt(mean(s^2)
+ * + eps) * weight, q / scales = the norm as MXFP8 rows. residual may be NULL
+ * (plain norm). sum_out and norm_out (fp32) may be NULL; sum_out may alias x
+ * or residual, norm_out may alias x. The norm is the exact value rounded to
+ * fp32 once (squares and inverse root in fp64), so it can differ from
+ * add_rms_norm's in the last bit, and the codes do not depend on summation
+ * order. n % 32 == 0, n <= 16384; fp32 buffers 16-byte aligned. */
+int ds3_cuda_add_rms_norm_mx(const ds3_cuda_buffer_t *x, const ds3_cuda_buffer_t *residual,
+                             const ds3_cuda_buffer_t *weight,
+                             ds3_cuda_buffer_t *sum_out, ds3_cuda_buffer_t *norm_out,
+                             ds3_cuda_buffer_t *q, ds3_cuda_buffer_t *scales,
+                             uint32_t n, uint32_t n_rows, float eps);
+
+/* Rows sorted by expert, without the list capacities of moe_expert_lists. idx
+ * int32 [n_tokens, n_used] (router output). offsets int32 [n_expert + 1]:
+ * expert e's rows are offsets[e] .. offsets[e+1]-1, and offsets[n_expert] is
+ * the number of rows. entries int32 [n_tokens * n_used]: row r stands for
+ * entry entries[r] = token * n_used + slot, ascending within an expert. row_of
+ * int32 [n_tokens * n_used] (or NULL) is the inverse map, usable as y_rows of
+ * moe_combine_residual. An expert id outside [0, n_expert) makes the call
+ * return -1, is left out of the rows and gets row_of -1; entries past
+ * offsets[n_expert] are not written. n_expert <= 256. */
+int ds3_cuda_moe_expert_rows(const ds3_cuda_buffer_t *idx, ds3_cuda_buffer_t *offsets, ds3_cuda_buffer_t *entries,
+                             ds3_cuda_buffer_t *row_of, uint32_t n_tokens, uint32_t n_expert, uint32_t n_used);
+
+/* Products grouped by expert with ragged sizes, on the tensor cores:
+ *   out[o(r)][m] = sum_k x[i(r)][k] * W_e[m][k]   for r in group e.
+ * offsets int32 [n_expert + 1] as moe_expert_rows writes it (any ascending
+ * bounds within [0, n_rows]; groups may be empty, rows past the last group are
+ * left as they were). x: MXFP8 [n_x][n_in]; i(r) = x_rows[r] / x_div (x_rows
+ * int32 [n_rows]; entries with x_div = n_used reads token rows), or r when
+ * x_rows is NULL (then n_x >= n_rows). w: MX rows [n_expert][n_out][n_in] of
+ * w_type. out: fp32 or fp16 rows of n_out (out_type); o(r) = out_rows[r]
+ * (int32 [n_rows]; entries puts results back in token order), or r when
+ * out_rows is NULL. Sums are fp32. n_in % 32 == 0 for MXFP8 weights, % 128 ==
+ * 0 for MXFP4. A row of x named outside [0, n_x) gives a zero row, an output
+ * row outside `out` is skipped, a bad offsets table is clamped; each makes the
+ * call return -1. With n_expert 1 and offsets {0, n_rows} it is a dense
+ * product. n_expert <= 256. */
+int ds3_cuda_moe_mx_matmul(const ds3_cuda_buffer_t *x_q, const ds3_cuda_buffer_t *x_scales,
+                           const ds3_cuda_buffer_t *x_rows, uint32_t x_div, const ds3_cuda_buffer_t *offsets,
+                           const ds3_cuda_buffer_t *w_q, const ds3_cuda_buffer_t *w_scales, ds3_cuda_mx_t w_type,
+                           ds3_cuda_buffer_t *out, ds3_type_t out_type, const ds3_cuda_buffer_t *out_rows,
+                           uint32_t n_x, uint32_t n_rows, uint32_t n_expert, uint32_t n_in, uint32_t n_out);
+
+/* The experts' gate and up products with SwiGLU in one pass, the result
+ * quantised for the down product:
+ *   h[r] = silu(gate(r)) * up(r) * row_weight[j(r)],  act_q / act_scales[r] = MXFP8(h[r]).
+ * Arguments as moe_mx_matmul; the gate and up weights are [n_expert][n_ff]
+ * [n_in] of one w_type. row_weight fp32 (or NULL): j(r) = x_rows[r] when x_rows
+ * is given (the router's scores [n_tokens, n_used] with entries), else r.
+ * act rows are the sorted rows [n_rows][n_ff]. n_ff % 32 == 0. */
+int ds3_cuda_moe_mx_swiglu(const ds3_cuda_buffer_t *x_q, const ds3_cuda_buffer_t *x_scales,
+                           const ds3_cuda_buffer_t *x_rows, uint32_t x_div, const ds3_cuda_buffer_t *offsets,
+                           const ds3_cuda_buffer_t *gate_q, const ds3_cuda_buffer_t *gate_scales,
+                           const ds3_cuda_buffer_t *up_q, const ds3_cuda_buffer_t *up_scales, ds3_cuda_mx_t w_type,
+                           const ds3_cuda_buffer_t *row_weight,
+                           ds3_cuda_buffer_t *act_q, ds3_cuda_buffer_t *act_scales,
+                           uint32_t n_x, uint32_t n_rows, uint32_t n_expert, uint32_t n_in, uint32_t n_ff);
+
+/* ------------------------------------------------------------------ */
 /* Copy lanes (new): host transfers that overlap the ops              */
 /* ------------------------------------------------------------------ */
 

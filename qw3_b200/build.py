@@ -19,7 +19,8 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libds3cuda.so"
-SOURCES = ["ds3_cuda.cu", "norm.cu", "embed.cu", "rope.cu", "router.cu", "moe.cu", "moe_route.cu", "router_gemv.cu", "gguf.cpp"]
+SOURCES = ["ds3_cuda.cu", "norm.cu", "embed.cu", "rope.cu", "router.cu", "moe.cu", "moe_route.cu", "router_gemv.cu", "mx.cu",
+           "moe_mx.cu", "gguf.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -66,7 +67,7 @@ def build(force: bool = False, ptxas_verbose: bool = False) -> Path:
         return LIB
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [
-        nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared",
+        nvcc(), *ARCH, "--threads", "0", "-O3", "-lineinfo", "-std=c++17", "-shared",
         "-Xcompiler", "-fPIC,-fvisibility=hidden", "-Xcompiler", "-O2",
         "-I", str(ROOT / "include"), "-I", str(CSRC),
         "-cudart", "static",

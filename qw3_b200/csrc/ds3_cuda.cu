@@ -1260,6 +1260,297 @@ int ds3_cuda_moe_combine_residual(const ds3_cuda_buffer_t *y, const ds3_cuda_buf
                   ps);
 }
 
+// ------------------------------------------------ MX rows, experts' products
+// These entries check their arguments before they look for a device.
+
+static bool aligned(const char *op, const char *name, const ds3_cuda_buffer_t *b, uintptr_t a)
+{
+    if (b && reinterpret_cast<uintptr_t>(dptr(b)) % a) {
+        set_error("%s: %s must be %u-byte aligned", op, name, (unsigned)a);
+        return false;
+    }
+    return true;
+}
+
+// `out` shares no byte with `in` (buffers that hold less than they use are refused before).
+static bool disjoint(const char *op, const char *out_name, const ds3_cuda_buffer_t *out, size_t out_bytes,
+                     const char *in_name, const ds3_cuda_buffer_t *in, size_t in_bytes)
+{
+    if (!out || !in || !out_bytes || !in_bytes) return true;
+    const char *o = (const char *)dptr(out), *i = (const char *)dptr(in);
+    if (o < i + in_bytes && i < o + out_bytes) {
+        set_error("%s: %s overlaps %s", op, out_name, in_name);
+        return false;
+    }
+    return true;
+}
+
+static bool mx_type(const char *op, ds3_cuda_mx_t t)
+{
+    if (t == DS3_CUDA_MXFP8 || t == DS3_CUDA_MXFP4) return true;
+    set_error("%s: type %d is not DS3_CUDA_MXFP8 or DS3_CUDA_MXFP4", op, (int)t);
+    return false;
+}
+
+// Elements of [rows][cols], bounded so that every byte count below fits.
+static bool mx_shape(const char *op, uint64_t rows, uint64_t cols, uint64_t *n)
+{
+    if (cols == 0 || cols % 32) {
+        set_error("%s: a row of %llu elements is not a whole number of 32-element blocks", op, (unsigned long long)cols);
+        return false;
+    }
+    if (rows > (1ull << 42) / cols) {
+        set_error("%s: %llu rows of %llu elements are too many", op, (unsigned long long)rows, (unsigned long long)cols);
+        return false;
+    }
+    *n = rows * cols;
+    return true;
+}
+
+static size_t mx_bytes(ds3_cuda_mx_t t, uint64_t n) { return (size_t)(t == DS3_CUDA_MXFP4 ? n / 2 : n); }
+
+int ds3_cuda_mx_quantize(const ds3_cuda_buffer_t *src, ds3_type_t src_type, ds3_cuda_buffer_t *q,
+                         ds3_cuda_buffer_t *scales, ds3_cuda_mx_t to, uint64_t n_rows, uint32_t n_cols)
+{
+    const char *op = "mx_quantize";
+    uint64_t n = 0;
+    if (!mx_type(op, to) || !mx_shape(op, n_rows, n_cols, &n)) return -1;
+    if ((int)src_type != 0 && (int)src_type != 1) {
+        set_error("%s: src_type must be DS3_TYPE_F32 or DS3_TYPE_F16", op);
+        return -1;
+    }
+    const size_t sb = (size_t)n * ((int)src_type == 1 ? 2 : 4), qb = mx_bytes(to, n), cb = (size_t)(n / 32);
+    if (!need(op, "src", src, sb) || !need(op, "q", q, qb) || !need(op, "scales", scales, cb) || !writable(op, "q", q) ||
+        !writable(op, "scales", scales) || !aligned(op, "src", src, 16) || !aligned(op, "q", q, 16) ||
+        !disjoint(op, "q", q, qb, "src", src, sb) || !disjoint(op, "scales", scales, cb, "src", src, sb) ||
+        !disjoint(op, "q", q, qb, "scales", scales, cb) || !ready(op))
+        return -1;
+    if (n == 0) return 0;
+    ProfScope ps(op);
+    return finish(op,
+                  ds3::launch_mx_quantize(ctx(), dptr(src), (int)src_type == 1, (uint8_t *)dptr(q),
+                                          (uint8_t *)dptr(scales), (int)to, (int64_t)n),
+                  ps);
+}
+
+int ds3_cuda_mx_dequantize(const ds3_cuda_buffer_t *q, const ds3_cuda_buffer_t *scales, ds3_cuda_mx_t from,
+                           ds3_cuda_buffer_t *dst, uint64_t n_rows, uint32_t n_cols)
+{
+    const char *op = "mx_dequantize";
+    uint64_t n = 0;
+    if (!mx_type(op, from) || !mx_shape(op, n_rows, n_cols, &n)) return -1;
+    const size_t qb = mx_bytes(from, n), cb = (size_t)(n / 32), db = (size_t)n * 4;
+    if (!need(op, "q", q, qb) || !need(op, "scales", scales, cb) || !need(op, "dst", dst, db) ||
+        !writable(op, "dst", dst) || !aligned(op, "q", q, 16) || !aligned(op, "dst", dst, 16) ||
+        !disjoint(op, "dst", dst, db, "q", q, qb) || !disjoint(op, "dst", dst, db, "scales", scales, cb) || !ready(op))
+        return -1;
+    if (n == 0) return 0;
+    ProfScope ps(op);
+    return finish(op,
+                  ds3::launch_mx_dequantize(ctx(), (const uint8_t *)dptr(q), (const uint8_t *)dptr(scales), (int)from,
+                                            (float *)dptr(dst), (int64_t)n),
+                  ps);
+}
+
+int ds3_cuda_add_rms_norm_mx(const ds3_cuda_buffer_t *x, const ds3_cuda_buffer_t *residual,
+                             const ds3_cuda_buffer_t *weight, ds3_cuda_buffer_t *sum_out, ds3_cuda_buffer_t *norm_out,
+                             ds3_cuda_buffer_t *q, ds3_cuda_buffer_t *scales, uint32_t n, uint32_t n_rows, float eps)
+{
+    const char *op = "add_rms_norm_mx";
+    uint64_t e = 0;
+    if (!mx_shape(op, n_rows, n, &e)) return -1;
+    if (n > 16384) {
+        set_error("%s: n %u exceeds 16384", op, n);
+        return -1;
+    }
+    const size_t rb = (size_t)e * 4, wb = (size_t)n * 4, qb = (size_t)e, cb = (size_t)(e / 32);
+    if (!need(op, "x", x, rb) || (residual && !need(op, "residual", residual, rb)) || !need(op, "weight", weight, wb) ||
+        (sum_out && (!need(op, "sum_out", sum_out, rb) || !writable(op, "sum_out", sum_out))) ||
+        (norm_out && (!need(op, "norm_out", norm_out, rb) || !writable(op, "norm_out", norm_out))) ||
+        !need(op, "q", q, qb) || !writable(op, "q", q) || !need(op, "scales", scales, cb) ||
+        !writable(op, "scales", scales) || !aligned(op, "x", x, 16) || !aligned(op, "residual", residual, 16) ||
+        !aligned(op, "weight", weight, 16) || !aligned(op, "sum_out", sum_out, 16) ||
+        !aligned(op, "norm_out", norm_out, 16) || !aligned(op, "q", q, 16))
+        return -1;
+    // A row's outputs may replace that row of x or the residual, whole; any other overlap is refused.
+    const bool sum_over_x = sum_out && dptr(sum_out) == dptr(x), norm_over_x = norm_out && dptr(norm_out) == dptr(x);
+    const bool sum_over_r = sum_out && residual && dptr(sum_out) == dptr(residual);
+    if ((!sum_over_x && !disjoint(op, "sum_out", sum_out, rb, "x", x, rb)) ||
+        (!sum_over_r && !disjoint(op, "sum_out", sum_out, rb, "residual", residual, rb)) ||
+        !disjoint(op, "sum_out", sum_out, rb, "weight", weight, wb) ||
+        (!norm_over_x && !disjoint(op, "norm_out", norm_out, rb, "x", x, rb)) ||
+        !disjoint(op, "norm_out", norm_out, rb, "residual", residual, rb) ||
+        !disjoint(op, "norm_out", norm_out, rb, "weight", weight, wb) ||
+        !disjoint(op, "norm_out", norm_out, rb, "sum_out", sum_out, rb) || !disjoint(op, "q", q, qb, "x", x, rb) ||
+        !disjoint(op, "q", q, qb, "residual", residual, rb) || !disjoint(op, "q", q, qb, "weight", weight, wb) ||
+        !disjoint(op, "q", q, qb, "sum_out", sum_out, rb) || !disjoint(op, "q", q, qb, "norm_out", norm_out, rb) ||
+        !disjoint(op, "scales", scales, cb, "x", x, rb) || !disjoint(op, "scales", scales, cb, "residual", residual, rb) ||
+        !disjoint(op, "scales", scales, cb, "weight", weight, wb) ||
+        !disjoint(op, "scales", scales, cb, "sum_out", sum_out, rb) ||
+        !disjoint(op, "scales", scales, cb, "norm_out", norm_out, rb) || !disjoint(op, "q", q, qb, "scales", scales, cb) ||
+        !ready(op))
+        return -1;
+    if (n_rows == 0) return 0;
+    ProfScope ps(op);
+    return finish(op,
+                  ds3::launch_add_rms_norm_mx(ctx(), (const float *)dptr(x), (const float *)dptr(residual),
+                                              (const float *)dptr(weight), (float *)dptr(sum_out),
+                                              (float *)dptr(norm_out), (uint8_t *)dptr(q), (uint8_t *)dptr(scales),
+                                              (int)n, n_rows, eps),
+                  ps);
+}
+
+int ds3_cuda_moe_expert_rows(const ds3_cuda_buffer_t *idx, ds3_cuda_buffer_t *offsets, ds3_cuda_buffer_t *entries,
+                             ds3_cuda_buffer_t *row_of, uint32_t n_tokens, uint32_t n_expert, uint32_t n_used)
+{
+    const char *op = "moe_expert_rows";
+    if (n_expert == 0 || n_expert > 256 || n_used == 0 || (uint64_t)n_tokens * n_used > (1u << 30)) {
+        set_error("%s: need 0 < n_expert <= 256, n_used > 0, n_tokens * n_used <= 2^30", op);
+        return -1;
+    }
+    const size_t ent = (size_t)n_tokens * n_used * 4, ob = ((size_t)n_expert + 1) * 4;
+    if (!need(op, "idx", idx, ent) || !need(op, "offsets", offsets, ob) || !writable(op, "offsets", offsets) ||
+        !need(op, "entries", entries, ent) || !writable(op, "entries", entries) ||
+        (row_of && (!need(op, "row_of", row_of, ent) || !writable(op, "row_of", row_of))) ||
+        !disjoint(op, "offsets", offsets, ob, "idx", idx, ent) || !disjoint(op, "entries", entries, ent, "idx", idx, ent) ||
+        !disjoint(op, "row_of", row_of, ent, "idx", idx, ent) ||
+        !disjoint(op, "entries", entries, ent, "offsets", offsets, ob) ||
+        !disjoint(op, "row_of", row_of, ent, "offsets", offsets, ob) ||
+        !disjoint(op, "row_of", row_of, ent, "entries", entries, ent) || !ready(op))
+        return -1;
+    ProfScope ps(op);
+    return finish(op,
+                  ds3::launch_moe_expert_rows(ctx(), (const int32_t *)dptr(idx), (int32_t *)dptr(offsets),
+                                              (int32_t *)dptr(entries), (int32_t *)dptr(row_of),
+                                              (int64_t)n_tokens * n_used, (int)n_expert),
+                  ps);
+}
+
+// Both grouped products: gate / up with SwiGLU when w1 is given.
+static int moe_mx_common(const char *op, const ds3_cuda_buffer_t *x_q, const ds3_cuda_buffer_t *x_s,
+                         const ds3_cuda_buffer_t *x_rows, uint32_t x_div, const ds3_cuda_buffer_t *offsets,
+                         const ds3_cuda_buffer_t *w0, const ds3_cuda_buffer_t *w0_s, bool swiglu,
+                         const ds3_cuda_buffer_t *w1, const ds3_cuda_buffer_t *w1_s, ds3_cuda_mx_t w_type,
+                         const ds3_cuda_buffer_t *row_weight, ds3_cuda_buffer_t *out, ds3_cuda_buffer_t *out_s,
+                         ds3_type_t out_type, const ds3_cuda_buffer_t *out_rows, uint32_t n_x, uint32_t n_rows,
+                         uint32_t n_expert, uint32_t n_in, uint32_t n_out)
+{
+    if (!mx_type(op, w_type)) return -1;
+    if (n_expert == 0 || n_expert > 256) {
+        set_error("%s: need 0 < n_expert (%u) <= 256", op, n_expert);
+        return -1;
+    }
+    if (x_rows && x_div == 0) {
+        set_error("%s: x_div must be > 0", op);
+        return -1;
+    }
+    if (n_x > 0x7fffffffu || n_rows > 0x7fffffffu || n_in > (1u << 24) || n_out > (1u << 24) ||
+        (x_rows && (uint64_t)n_x * x_div > 0x7fffffffu)) {
+        set_error("%s: n_x, n_rows or n_x * x_div exceeds 2^31 - 1, or n_in or the row length 2^24", op);
+        return -1;
+    }
+    const uint32_t k_step = w_type == DS3_CUDA_MXFP4 ? 128 : 32;
+    if (n_in == 0 || n_in % k_step || n_out == 0 || (swiglu && n_out % 32)) {
+        set_error("%s: n_in %u must be a multiple of %u%s", op, n_in, k_step,
+                  swiglu ? " and n_ff one of 32" : " and n_out > 0");
+        return -1;
+    }
+    if (!swiglu && (int)out_type != 0 && (int)out_type != 1) {
+        set_error("%s: out_type must be DS3_TYPE_F32 or DS3_TYPE_F16", op);
+        return -1;
+    }
+    uint64_t nx = 0, nw = 0;
+    if (!mx_shape(op, n_x, n_in, &nx) || !mx_shape(op, (uint64_t)n_expert * n_out, n_in, &nw)) return -1;
+    const size_t es = swiglu ? 1 : (int)out_type == 1 ? 2 : 4;
+    const size_t xb = (size_t)nx, xsb = (size_t)(nx / 32), wb = mx_bytes(w_type, nw), wsb = (size_t)(nw / 32);
+    const size_t rb = (size_t)n_rows * 4, ofb = ((size_t)n_expert + 1) * 4;
+    const size_t row = (size_t)n_out * es;
+    const size_t rwb = (x_rows ? (size_t)n_x * x_div : (size_t)n_rows) * 4;
+    if (!need(op, "x_q", x_q, xb) || !need(op, "x_scales", x_s, xsb) || !need(op, "offsets", offsets, ofb) ||
+        (x_rows && !need(op, "x_rows", x_rows, rb)) || (out_rows && !need(op, "out_rows", out_rows, rb)) ||
+        !need(op, swiglu ? "gate_q" : "w_q", w0, wb) || !need(op, swiglu ? "gate_scales" : "w_scales", w0_s, wsb) ||
+        (swiglu && (!need(op, "up_q", w1, wb) || !need(op, "up_scales", w1_s, wsb))) ||
+        (row_weight && !need(op, "row_weight", row_weight, rwb)))
+        return -1;
+    // Without a row map out holds n_rows rows; with one, the rows it has.
+    const char *on = swiglu ? "act_q" : "out";
+    if (!need(op, on, out, out_rows ? row : (size_t)n_rows * row) || !writable(op, on, out)) return -1;
+    const uint64_t n_out_rows = out_rows ? out->bytes / row : n_rows;
+    const size_t outb = (size_t)n_out_rows * row, osb = (size_t)n_rows * (n_out / 32);
+    if (swiglu && (!need(op, "act_scales", out_s, osb) || !writable(op, "act_scales", out_s))) return -1;
+    if (!x_rows && n_x < n_rows) {
+        set_error("%s: without x_rows, x needs n_rows (%u) rows and has %u", op, n_rows, n_x);
+        return -1;
+    }
+    const uintptr_t wa = w_type == DS3_CUDA_MXFP4 ? 32 : 16;
+    if (!aligned(op, "x_q", x_q, 16) || !aligned(op, swiglu ? "gate_q" : "w_q", w0, wa) || !aligned(op, "up_q", w1, wa) ||
+        !aligned(op, on, out, es) || !aligned(op, "offsets", offsets, 4) || !aligned(op, "x_rows", x_rows, 4) ||
+        !aligned(op, "out_rows", out_rows, 4) || !aligned(op, "row_weight", row_weight, 4))
+        return -1;
+    const struct {
+        const char *name;
+        const ds3_cuda_buffer_t *b;
+        size_t bytes;
+    } ins[] = {{"x_q", x_q, xb},          {"x_scales", x_s, xsb},       {"x_rows", x_rows, rb}, {"offsets", offsets, ofb},
+               {"weights", w0, wb},       {"weight scales", w0_s, wsb}, {"up_q", w1, wb},       {"up_scales", w1_s, wsb},
+               {"out_rows", out_rows, rb}, {"row_weight", row_weight, rwb}};
+    for (const auto &i : ins)
+        if (!disjoint(op, on, out, outb, i.name, i.b, i.bytes) ||
+            !disjoint(op, "act_scales", out_s, osb, i.name, i.b, i.bytes))
+            return -1;
+    if (!disjoint(op, on, out, outb, "act_scales", out_s, osb) || !ready(op)) return -1;
+    if (n_rows == 0) return 0;
+    if (n_x == 0) {
+        set_error("%s: n_rows is %u but x has no rows", op, n_rows);
+        return -1;
+    }
+    ds3::MoeMxCall c = {};
+    c.x = (const uint8_t *)dptr(x_q);
+    c.x_s = (const uint8_t *)dptr(x_s);
+    c.x_rows = (const int32_t *)dptr(x_rows);
+    c.offsets = (const int32_t *)dptr(offsets);
+    c.w0 = (const uint8_t *)dptr(w0);
+    c.w0_s = (const uint8_t *)dptr(w0_s);
+    c.w1 = (const uint8_t *)dptr(w1);
+    c.w1_s = (const uint8_t *)dptr(w1_s);
+    c.row_w = (const float *)dptr(row_weight);
+    c.out_rows = (const int32_t *)dptr(out_rows);
+    c.out = dptr(out);
+    c.out_s = (uint8_t *)dptr(out_s);
+    c.w_type = (int)w_type;
+    c.n_x = (int)n_x;
+    c.x_div = x_rows ? (int)x_div : 1;
+    c.n_rows = (int)n_rows;
+    c.n_out_rows = (int)(n_out_rows < 0x7fffffffu ? n_out_rows : 0x7fffffffu);
+    c.n_group = (int)n_expert;
+    c.K = (int)n_in;
+    c.n_w = (int)n_out;
+    c.out_f16 = !swiglu && (int)out_type == 1;
+    ProfScope ps(op);
+    return finish(op, ds3::launch_moe_mx(ctx(), c), ps);
+}
+
+int ds3_cuda_moe_mx_matmul(const ds3_cuda_buffer_t *x_q, const ds3_cuda_buffer_t *x_scales,
+                           const ds3_cuda_buffer_t *x_rows, uint32_t x_div, const ds3_cuda_buffer_t *offsets,
+                           const ds3_cuda_buffer_t *w_q, const ds3_cuda_buffer_t *w_scales, ds3_cuda_mx_t w_type,
+                           ds3_cuda_buffer_t *out, ds3_type_t out_type, const ds3_cuda_buffer_t *out_rows, uint32_t n_x,
+                           uint32_t n_rows, uint32_t n_expert, uint32_t n_in, uint32_t n_out)
+{
+    return moe_mx_common("moe_mx_matmul", x_q, x_scales, x_rows, x_div, offsets, w_q, w_scales, false, nullptr, nullptr,
+                         w_type, nullptr, out, nullptr, out_type, out_rows, n_x, n_rows, n_expert, n_in, n_out);
+}
+
+int ds3_cuda_moe_mx_swiglu(const ds3_cuda_buffer_t *x_q, const ds3_cuda_buffer_t *x_scales,
+                           const ds3_cuda_buffer_t *x_rows, uint32_t x_div, const ds3_cuda_buffer_t *offsets,
+                           const ds3_cuda_buffer_t *gate_q, const ds3_cuda_buffer_t *gate_scales,
+                           const ds3_cuda_buffer_t *up_q, const ds3_cuda_buffer_t *up_scales, ds3_cuda_mx_t w_type,
+                           const ds3_cuda_buffer_t *row_weight, ds3_cuda_buffer_t *act_q, ds3_cuda_buffer_t *act_scales,
+                           uint32_t n_x, uint32_t n_rows, uint32_t n_expert, uint32_t n_in, uint32_t n_ff)
+{
+    return moe_mx_common("moe_mx_swiglu", x_q, x_scales, x_rows, x_div, offsets, gate_q, gate_scales, true, up_q, up_scales,
+                         w_type, row_weight, act_q, act_scales, DS3_TYPE_F32, nullptr, n_x, n_rows, n_expert, n_in, n_ff);
+}
+
 // ------------------------------------------------------------- copy lanes
 static cudaStream_t lane_stream(const char *op, int lane)
 {

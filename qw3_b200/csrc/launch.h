@@ -96,6 +96,33 @@ cudaError_t launch_moe_expert_lists(const LaunchCtx &c, const int32_t *idx, cons
                                     int32_t *ids, float *gscores, int32_t *slot_of, int64_t n_tokens, int n_used,
                                     int n_expert, int64_t cap);
 
+// fp32 / fp16 rows (n elements in all, a multiple of 32) to MX rows and back (mx.cu).
+cudaError_t launch_mx_quantize(const LaunchCtx &c, const void *src, bool f16, uint8_t *q, uint8_t *scales, int to, int64_t n);
+cudaError_t launch_mx_dequantize(const LaunchCtx &c, const uint8_t *q, const uint8_t *scales, int from, float *dst, int64_t n);
+// x [rows, n] (+ r) -> sum_out, norm_out (either may be null) and MXFP8 rows of the norm.
+cudaError_t launch_add_rms_norm_mx(const LaunchCtx &c, const float *x, const float *r, const float *w, float *sum_out,
+                                   float *norm_out, uint8_t *q, uint8_t *scales, int n, int64_t rows, float eps);
+// Rows sorted by expert: offsets, entries and their inverse (moe_route.cu).
+cudaError_t launch_moe_expert_rows(const LaunchCtx &c, const int32_t *idx, int32_t *offsets, int32_t *entries,
+                                   int32_t *row_of, int64_t n_entries, int n_expert);
+
+// Products grouped by expert over MX rows (moe_mx.cu). w1 != nullptr: SwiGLU
+// of the w0 (gate) and w1 (up) products to MXFP8 rows; else the w0 product,
+// fp32 or fp16. Pointers and sizes as the public entries check them.
+struct MoeMxCall {
+    const uint8_t *x, *x_s;           // MXFP8 rows [n_x][K], scales [n_x][K/32]
+    const int32_t *x_rows;            // [n_rows] or nullptr
+    const int32_t *offsets;           // [n_group + 1]
+    const uint8_t *w0, *w0_s, *w1, *w1_s;
+    const float *row_w;
+    const int32_t *out_rows;          // [n_rows] or nullptr
+    void *out;
+    uint8_t *out_s;
+    int w_type, n_x, x_div, n_rows, n_out_rows, n_group, K, n_w;
+    bool out_f16;
+};
+cudaError_t launch_moe_mx(const LaunchCtx &c, const MoeMxCall &q);
+
 cudaError_t launch_bounded_wait_selftest(const LaunchCtx &c, uint32_t polls);
 // Compute capability (major*10 + minor) of the loaded kernel code, or -1.
 int kernel_binary_version();

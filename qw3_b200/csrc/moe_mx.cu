@@ -1,0 +1,795 @@
+// Matrix products grouped by expert over microscaled (MX) rows, on the
+// tensor cores (sm_100a): the experts' gate / up products fused with SwiGLU
+// and the 8-bit quantisation of its result, and the plain product (the
+// experts' down projection).
+//
+// The engine runs them per expert (forward_chunk_post_gathered,
+// src/ds3_engine.c:973-1011: gather the expert's token rows, gate and up
+// products, silu_mul, down product); here one launch covers all experts.
+//
+// Mathematics. Rows are sorted by expert; group e is rows
+// offsets[e] .. offsets[e+1]-1. For row r of group e, with x = MXFP8 and W_e =
+// MXFP8 or MXFP4 (value = element * 2^(scale-127), one scale per 32 elements):
+//   y[r][m] = sum_k x[r][k] * W_e[m][k]
+// and for SwiGLU, with G = gate and U = up products:
+//   h[r][f] = silu(G[r][f]) * U[r][f] * row_weight,   act = MXFP8(h)
+//
+// Tiling. The weight rows take the 128-row side of the tensor-core tile (A)
+// and the tokens the free side (B, N <= NT columns), so a group of any size
+// wastes at most 15 columns: the instruction's N is set per tile to the
+// group's remaining rows rounded up to 16. A persistent CTA walks tiles
+// (expert, token block, weight block); the weight block is the fastest index,
+// so the CTAs working at the same time share token rows and, with several
+// token blocks, weights through L2. The tile list is derived on the device
+// from `offsets`; the host never reads it.
+//   - 128 K elements per stage: A 16 KB, B NT x 128 B, both in the 128-byte
+//     swizzle, one 32-bit word of four scales per row.
+//   - tcgen05.mma kind::mxf8f6f4 with block scales, K = 32 per instruction,
+//     accumulators fp32 in tensor memory, double buffered so the epilogue of
+//     one tile runs under the products of the next. Element products and
+//     scaling are exact; the only roundings are the fp32 accumulation's.
+//   - MXFP4 weights are expanded to one byte per element by the copy engine
+//     (packed in HBM, 16 elements per 16 bytes in shared memory).
+//   - SwiGLU's A tile is 64 gate rows over the same 64 up rows, so the four
+//     epilogue warps (one per 32 tensor-memory lanes) pair up: gate and up meet
+//     through a shared-memory exchange, and a warp's 32 lanes are the 32
+//     elements of one MX block.
+//
+// Warps: 0 copies (weights: tiled boxes; token rows: tiled boxes when
+// they are used in place), 1 issues the tensor-
+// core work, 2 / 3 stage the scales of A / B in the order the tensor core
+// wants them (row r of 128 -> lane r%32, word r/32), 4-11 are the epilogue,
+// and 12-15 gather token rows that come through x_rows.
+// Every wait is bounded; on a timeout the CTA records it, lets its copies and
+// products land (bounded), frees its tensor memory and returns.
+#include "common.cuh"
+#include "launch.h"
+#include "mx.cuh"
+
+#include <cuda.h>
+#include <cuda_fp16.h>
+
+namespace ds3 {
+namespace {
+
+constexpr int kTileM = 128;     // weight rows per tile
+constexpr int kStageK = 128;    // K elements per stage
+constexpr int kEpilogueThreads = 256, kGatherThreads = 128;
+constexpr int moe_threads(bool gather) { return 128 + kEpilogueThreads + (gather ? kGatherThreads : 0); }
+constexpr int kMaxGroups = 256;
+
+// Stages for NT token columns, as many as fit beside the exchange buffers.
+template <int NT>
+struct MoeLayout {
+    static constexpr int kStages = NT == 64 ? 8 : NT == 128 ? 6 : 4;
+    static constexpr int kABytes = kTileM * kStageK;
+    static constexpr int kBBytes = NT * kStageK;
+    static constexpr int kBWords = (NT + 127) / 128 * 4;  // tensor-memory columns of B's scales
+    static constexpr int kSfA = 512, kSfB = kBWords * 128;
+    static constexpr int kXch = 8 * 2 * 8 * 32 * 4;       // [epilogue warp][buffer][8][32] floats
+    static constexpr int kOffA = 0;
+    static constexpr int kOffB = kOffA + kStages * kABytes;
+    static constexpr int kOffSfA = kOffB + kStages * kBBytes;
+    static constexpr int kOffSfB = kOffSfA + kStages * kSfA;
+    static constexpr int kOffXch = kOffSfB + kStages * kSfB;
+    static constexpr int kOffTab = kOffXch + kXch;        // offsets and tile prefix
+    static constexpr int kOffIds = kOffTab + 2 * (kMaxGroups + 2) * 4;  // gathered row ids, per gathering warp
+    static constexpr int kUsed = kOffIds + 4 * NT * 4;
+    static constexpr size_t kSmem = kUsed + 1024;         // the base is aligned up to 1024
+    static constexpr int kSfCols = 4 + kBWords;
+    static constexpr int kColsUsed = 2 * NT + kStages * kSfCols;
+    static constexpr int kTmemCols = kColsUsed <= 256 ? 256 : 512;
+    static_assert(kColsUsed <= 512 && kSmem <= 232448 - 512, "layout");
+};
+
+struct MoeMaps {
+    CUtensorMap w0, w1, x;
+};
+
+struct MoeArgs {
+    const uint8_t *x;          // [n_x][K]
+    const uint8_t *x_s;        // [n_x][K/32]
+    const uint8_t *w0_s, *w1_s;  // [E][n_w][K/32]
+    const int32_t *offsets;    // [E+1]
+    const int32_t *x_rows;     // sorted row -> x_div * (x row) + slot, or nullptr
+    const float *row_w;        // SwiGLU weight by x_rows' value (or row), or nullptr
+    const int32_t *out_rows;   // sorted row -> output row, or nullptr
+    void *out;                 // fp32 / fp16 [n_out_rows][n_w], or e4m3 [n_rows][n_w]
+    uint8_t *out_s;            // SwiGLU: [n_rows][n_w/32]
+    int n_x, n_rows, n_out_rows, n_group, x_div, K, n_w;
+    int x_vec, w_vec;          // widest aligned scale load: 16, 8, 4 or 1 bytes
+    int half, fp4;             // out is fp16; the weights are MXFP4
+};
+
+// ------------------------------------------------------------ PTX wrappers
+__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *m, int x, int y, int z, uint64_t *bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+            "r"(smem_addr(dst)), "l"(m), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *m, int x, int y, uint64_t *bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
+            "r"(smem_addr(dst)), "l"(m), "r"(x), "r"(y), "r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// Arrive on `bar` once this thread's earlier cp.async copies have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t *bar)
+{
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// Arrive on `bar` once all tensor-core work this thread issued has finished.
+__device__ __forceinline__ void tc_commit(uint64_t *bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+                 : "memory");
+}
+// 32 rows of 16 bytes, shared -> tensor memory, into all four lane quarters.
+__device__ __forceinline__ void tc_copy_scales(uint32_t tmem, uint64_t desc)
+{
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void tc_mma_mx(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,
+                                          uint32_t sfb, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::
+            "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tc_ld16(uint32_t (&v)[16], uint32_t tmem)
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(tmem)
+        : "memory");
+}
+// Shared-memory writes by threads (scales, gathered rows) that this thread has
+// seen through a barrier are seen by the tensor-core work it issues after this.
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// Whether `ok` holds in all `threads` threads that meet at barrier `id`.
+__device__ __forceinline__ bool named_all(int id, int threads, bool ok)
+{
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.and.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r) : "r"((uint32_t)ok), "r"(id), "r"(threads) : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ void named_sync(int id, int threads)
+{
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// Shared-memory matrix descriptor: start and stride-byte-offset in 16-byte
+// units, descriptor version 1, swizzle code `sw` (2 = 128 bytes, 0 = none).
+// K-major 128-byte-swizzled operand: 8-row groups 1024 bytes apart. Scales:
+// 8-row groups of 16-byte rows, 128 bytes apart.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t stride_bytes, uint64_t sw)
+{
+    return (uint64_t)((addr & 0x3ffffu) >> 4) | (1ull << 16) | ((uint64_t)(stride_bytes >> 4) << 32) | (1ull << 46) |
+           (sw << 61);
+}
+
+// 16 scales [16 g, 16 g + 16) of one row (those past n are 0). The widest
+// load that the base and the row stride allow; activations' scales bypass L1.
+__device__ __forceinline__ uint4 load_scales(const uint8_t *row, int g, int n, int vec)
+{
+    const uint8_t *p = row + 16 * g;
+    const int left = n - 16 * g;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (vec == 16) return __ldcg(reinterpret_cast<const uint4 *>(p));
+    if (vec == 8) {
+        const uint2 a = __ldcg(reinterpret_cast<const uint2 *>(p));
+        v.x = a.x;
+        v.y = a.y;
+        if (left > 8) {
+            const uint2 b = __ldcg(reinterpret_cast<const uint2 *>(p + 8));
+            v.z = b.x;
+            v.w = b.y;
+        }
+        return v;
+    }
+    if (vec == 4) {
+        const unsigned *q = reinterpret_cast<const unsigned *>(p);
+        v.x = __ldcg(q);
+        if (left > 4) v.y = __ldcg(q + 1);
+        if (left > 8) v.z = __ldcg(q + 2);
+        if (left > 12) v.w = __ldcg(q + 3);
+        return v;
+    }
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+        if (i < left) w[i >> 2] |= (uint32_t)__ldcg(p + i) << (8 * (i & 3));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint32_t word_of(const uint4 &v, int i)
+{
+    return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
+
+struct Tile {
+    int e, mt, n0, rows, r0;  // group, weight block, first row in the group, rows here, first sorted row
+};
+
+template <int NT>
+__device__ __forceinline__ Tile find_tile(const int *off, const int *pre, int n_group, int n_mt, int t)
+{
+    int lo = 0, hi = n_group;  // pre[lo] <= t < pre[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (pre[mid] <= t) lo = mid;
+        else hi = mid;
+    }
+    const int local = t - pre[lo];
+    Tile q;
+    q.e = lo;
+    q.mt = local % n_mt;
+    q.n0 = local / n_mt * NT;
+    const int cnt = off[lo + 1] - off[lo];
+    q.rows = cnt - q.n0 < NT ? cnt - q.n0 : NT;
+    q.r0 = off[lo] + q.n0;
+    return q;
+}
+
+// One warp stages the scales of J x 32 operand rows for every stage of every
+// tile of this CTA. Lane l owns rows l, l + 32, ...: it loads 16 scales (4
+// stages' worth) of each at a time, kAhead loads ahead of their use, and
+// stores word i of its rows side by side, which is the tensor core's order.
+constexpr int kAhead = 2;
+
+template <int J, int BYTES, int ST, typename Rows>
+__device__ __forceinline__ bool stage_scales(Rows rows_of, uint8_t *dst, uint64_t *full, uint64_t *empty, int total,
+                                             int n_kb, int nk32, int vec, int lane)
+{
+    const int n_groups = (n_kb + 3) >> 2;
+    const uint8_t *row[J];
+    uint4 buf[kAhead + 1][J];
+    // Load cursor (tile, group), kAhead groups in front of the store cursor.
+    int lt = blockIdx.x, lg = 0;
+    auto load_next = [&](uint4 (&v)[J]) {
+        if (lt < total) {
+            if (lg == 0) rows_of(row, lt);
+#pragma unroll
+            for (int j = 0; j < J; j++) v[j] = load_scales(row[j], lg, nk32, vec);
+        }
+        if (++lg == n_groups) {
+            lg = 0;
+            lt += gridDim.x;
+        }
+    };
+    int s = 0, g = 0, t = blockIdx.x;
+    uint32_t ph = 0;
+#pragma unroll
+    for (int i = 0; i < kAhead; i++) load_next(buf[i]);
+    while (t < total) {
+#pragma unroll
+        for (int u = 0; u <= kAhead; u++) {
+            load_next(buf[(u + kAhead) % (kAhead + 1)]);
+            if (t < total) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if (4 * g + i >= n_kb) break;
+                    if (!__all_sync(kFull, mbar_wait(&empty[s], ph ^ 1u, kWaitLimit))) return false;
+#pragma unroll
+                    for (int j = 0; j < J; j += 4) {
+                        uint4 w;
+                        w.x = word_of(buf[u][j], i);
+                        w.y = j + 1 < J ? word_of(buf[u][j + 1 < J ? j + 1 : 0], i) : 0u;
+                        w.z = j + 2 < J ? word_of(buf[u][j + 2 < J ? j + 2 : 0], i) : 0u;
+                        w.w = j + 3 < J ? word_of(buf[u][j + 3 < J ? j + 3 : 0], i) : 0u;
+                        *reinterpret_cast<uint4 *>(dst + s * BYTES + j * 128 + lane * 16) = w;
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&full[s]);
+                    if (++s == ST) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                }
+                if (++g == n_groups) {
+                    g = 0;
+                    t += gridDim.x;
+                }
+            }
+        }
+    }
+    return true;
+}
+
+// SWIGLU: w0 / w1 are the gate / up weights and out is MXFP8. Otherwise w0
+// alone, and out is fp32 or fp16. GATHER: token rows come through x_rows;
+// otherwise sorted row r is row r of x.
+template <int NT, bool SWIGLU, bool GATHER>
+__global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_constant__ MoeMaps maps, const MoeArgs a,
+                                                           unsigned *err)
+{
+    using L = MoeLayout<NT>;
+    constexpr int ST = L::kStages;
+    constexpr int kRowsPerTile = SWIGLU ? kTileM / 2 : kTileM;  // output columns per tile
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *sm = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+    __shared__ __align__(8) uint64_t full[ST], empty[ST], acc_full[2], acc_empty[2], drain;
+    __shared__ uint32_t tmem_base;
+    __shared__ int wsum[16];
+    int *off = reinterpret_cast<int *>(sm + L::kOffTab);
+    int *pre = off + kMaxGroups + 1;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int s = 0; s < ST; s++) {
+            // the copy thread, the two scale warps and each lane of one gathering warp
+            mbar_init(&full[s], 3 + (GATHER ? 32 : 0));
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(&acc_full[b], 1);
+            mbar_init(&acc_empty[b], kEpilogueThreads / 32);
+        }
+        mbar_init(&drain, 1);
+        mbar_init_fence();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)),
+                     "r"(L::kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pdl_wait();
+    pdl_trigger();
+
+    // Group bounds, clamped to 0 <= off[e] <= off[e+1] <= n_rows (a bad table
+    // is reported and never read past), and the tile prefix.
+    const int n_mt = (a.n_w + kRowsPerTile - 1) / kRowsPerTile;
+    {
+        int lo = 0, hi = 0;
+        if (tid < a.n_group) {
+            const int l0 = a.offsets[tid], h0 = a.offsets[tid + 1];
+            lo = min(max(l0, 0), a.n_rows);
+            hi = min(max(h0, lo), a.n_rows);
+            if ((lo != l0 || hi != h0) && blockIdx.x == 0) flag_error(err, kErrBadId);
+        }
+        int v = (hi - lo + NT - 1) / NT * n_mt;
+        int inc = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(kFull, inc, o);
+            if (lane >= o) inc += y;
+        }
+        if (lane == 31) wsum[warp] = inc;
+        __syncthreads();
+        int base = 0;
+        for (int i = 0; i < warp; i++) base += wsum[i];
+        if (tid < a.n_group) {
+            off[tid] = lo;
+            pre[tid] = base + inc - v;
+            if (tid == a.n_group - 1) {
+                off[tid + 1] = hi;
+                pre[tid + 1] = base + inc;
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const int total = pre[a.n_group];
+    const uint32_t tmem = tmem_base;
+    const int n_kb = (a.K + kStageK - 1) / kStageK;
+    const int nk32 = a.K / kMxBlock;
+    bool ok = true;
+    auto give_up = [&] { flag_error(err, kErrWaitTimeout); };
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ copies
+        // One thread runs the whole loop: per stage a wait, the byte count and
+        // the copies, without warp votes in between.
+        if (elect_one()) {
+            int s = 0, issued = 0;
+            uint32_t ph = 0;
+            for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+                const Tile q = find_tile<NT>(off, pre, a.n_group, n_mt, t);
+                const int nbox = GATHER ? 0 : (q.rows + 31) >> 5;
+                const uint32_t bytes = (a.fp4 ? L::kABytes / 2 : L::kABytes) + nbox * 4096;
+                const int row = q.mt * kRowsPerTile;
+                for (int kb = 0; kb < n_kb; kb++) {
+                    ok = mbar_wait(&empty[s], ph ^ 1u, kWaitLimit);
+                    if (!ok) break;
+                    uint8_t *A = sm + L::kOffA + s * L::kABytes, *B = sm + L::kOffB + s * L::kBBytes;
+                    mbar_expect_tx(&full[s], bytes);
+                    tma_load_3d(A, &maps.w0, kb * kStageK, row, q.e, &full[s]);
+                    if (SWIGLU) tma_load_3d(A + L::kABytes / 2, &maps.w1, kb * kStageK, row, q.e, &full[s]);
+                    if (!GATHER)
+                        for (int i = 0; i < nbox; i++)
+                            tma_load_2d(B + i * 4096, &maps.x, kb * kStageK, q.r0 + 32 * i, &full[s]);
+                    issued++;
+                    if (++s == ST) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                }
+            }
+            if (!ok) {
+                give_up();
+                // Let the copies in flight land before shared memory goes away.
+                for (int i = 0; i < ST && i < issued; i++) {
+                    if (s == 0) ph ^= 1u;
+                    s = s == 0 ? ST - 1 : s - 1;
+                    mbar_wait(&full[s], ph, kWaitLimit);
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ------------------------------------------------------ tensor cores
+        if (elect_one()) {
+            int s = 0, it = 0;
+            uint32_t ph = 0;
+            // A's type (5 = e2m1, 0 = e4m3), power-of-two scales, M.
+            const uint32_t idesc0 = ((a.fp4 ? 5u : 0u) << 7) | (1u << 23) | ((kTileM >> 4) << 24);
+            constexpr uint32_t kNextScale = (1u << 4) | (1u << 29);  // scale byte i of the word, B and A
+            const uint64_t ad0 = smem_desc(smem_addr(sm + L::kOffA), 1024, 2);
+            const uint64_t bd0 = smem_desc(smem_addr(sm + L::kOffB), 1024, 2);
+            const uint64_t sa0 = smem_desc(smem_addr(sm + L::kOffSfA), 128, 0);
+            const uint64_t sb0 = smem_desc(smem_addr(sm + L::kOffSfB), 128, 0);
+            for (int t = blockIdx.x; t < total && ok; t += gridDim.x, it++) {
+                const Tile q = find_tile<NT>(off, pre, a.n_group, n_mt, t);
+                const int b = it & 1;
+                ok = mbar_wait(&acc_empty[b], ((it >> 1) & 1u) ^ 1u, kWaitLimit);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t idesc = idesc0 | ((uint32_t)((q.rows + 15) >> 4) << 18);  // N / 8 at bit 17
+                const uint32_t d = tmem + b * NT;
+                for (int kb = 0; kb < n_kb; kb++) {
+                    ok = mbar_wait(&full[s], ph, kWaitLimit);
+                    if (!ok) break;
+                    tc_fence_after();
+                    fence_async_shared();
+                    const uint32_t sfa = tmem + 2 * NT + s * L::kSfCols, sfb = sfa + 4;
+                    tc_copy_scales(sfa, sa0 + s * (L::kSfA >> 4));
+#pragma unroll
+                    for (int j = 0; j < L::kBWords / 4; j++)
+                        tc_copy_scales(sfb + 4 * j, sb0 + s * (L::kSfB >> 4) + j * 32);
+                    const uint64_t ad = ad0 + s * (L::kABytes >> 4), bd = bd0 + s * (L::kBBytes >> 4);
+                    const int nk = nk32 - 4 * kb;  // 32-element steps left
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (i < nk)
+                            tc_mma_mx(d, ad + 2 * i, bd + 2 * i, idesc + i * kNextScale, sfa, sfb, (uint32_t)(kb | i));
+                    tc_commit(&empty[s]);
+                    if (++s == ST) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                }
+                if (ok) tc_commit(&acc_full[b]);
+            }
+            if (!ok) {
+                give_up();
+                tc_commit(&drain);  // products in flight finish before tensor memory is freed
+                mbar_wait(&drain, 0, kWaitLimit);
+            }
+        }
+        __syncwarp();
+    } else if (warp < 4) {
+        // ------------------------------------------------------------ scales
+        auto rows_of_a = [&](const uint8_t *(&row)[4], int t) {
+            const Tile q = find_tile<NT>(off, pre, a.n_group, n_mt, t);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int r = min(q.mt * kRowsPerTile + 32 * (SWIGLU ? j & 1 : j) + lane, a.n_w - 1);
+                row[j] = (SWIGLU && j >= 2 ? a.w1_s : a.w0_s) + ((size_t)q.e * a.n_w + r) * nk32;
+            }
+        };
+        auto rows_of_b = [&](const uint8_t *(&row)[NT / 32], int t) {
+            const Tile q = find_tile<NT>(off, pre, a.n_group, n_mt, t);
+#pragma unroll
+            for (int j = 0; j < NT / 32; j++) {
+                int x = q.r0 + min(lane + 32 * j, q.rows - 1);
+                if (a.x_rows) {
+                    x = a.x_rows[x];
+                    x = x < 0 ? -1 : x / a.x_div;
+                    x = x < 0 || x >= a.n_x ? 0 : x;
+                }
+                row[j] = a.x_s + (size_t)x * nk32;
+            }
+        };
+        ok = warp == 2 ? stage_scales<4, L::kSfA, ST>(rows_of_a, sm + L::kOffSfA, full, empty, total, n_kb, nk32, a.w_vec, lane)
+                       : stage_scales<NT / 32, L::kSfB, ST>(rows_of_b, sm + L::kOffSfB, full, empty, total, n_kb, nk32,
+                                                           a.x_vec, lane);
+        if (!ok) give_up();
+    } else if (GATHER && warp >= 12) {
+        // ------------------------------------------------------- row gathers
+        // Warp g fills stages g, g + 4, ... of the CTA's sequence. Eight lanes
+        // copy a token row's 128 bytes, four rows per instruction.
+        const int g = warp - 12, piece = lane & 7, r4 = lane >> 3;
+        int *id = reinterpret_cast<int *>(sm + L::kOffIds) + g * NT;
+        int nid[NT / 32];
+        auto rows_of = [&](int t) {
+            const Tile q = find_tile<NT>(off, pre, a.n_group, n_mt, t);
+#pragma unroll
+            for (int j = 0; j < NT / 32; j++) {
+                const int r = min(lane + 32 * j, q.rows - 1);
+                // A row id outside x reads row 0; the epilogue zeroes it.
+                int x = a.x_rows[q.r0 + r];
+                x = x < 0 ? -1 : x / a.x_div;
+                nid[j] = x < 0 || x >= a.n_x ? 0 : x;
+            }
+            return q.rows;
+        };
+        int t = blockIdx.x, seq = 0, rows = 0;  // seq: stages of this CTA before the tile
+        if (t < total) rows = rows_of(t);
+        for (; t < total && ok; t += gridDim.x) {
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < NT / 32; j++) id[lane + 32 * j] = nid[j];
+            __syncwarp();
+            const int n = rows;
+            if (t + (int)gridDim.x < total) rows = rows_of(t + gridDim.x);
+            for (int kb = (g - seq) & 3; kb < n_kb; kb += 4) {
+                const int s = (seq + kb) % ST;
+                ok = __all_sync(kFull, mbar_wait(&empty[s], ((uint32_t)(seq + kb) / ST & 1u) ^ 1u, kWaitLimit));
+                if (!ok) break;
+                const uint32_t dst = smem_addr(sm + L::kOffB + s * L::kBBytes) + r4 * 128;
+                const uint8_t *src = a.x + kb * kStageK + piece * 16;
+                if (kb * kStageK + piece * 16 < a.K) {
+#pragma unroll 4
+                    for (int i = 0; i < n; i += 4)  // the 128-byte swizzle: piece ^ (row % 8)
+                        cp_async16(dst + i * 128 + ((piece ^ ((i + r4) & 7)) << 4),
+                                   src + (size_t)(uint32_t)id[i + r4] * (uint32_t)a.K);
+                }
+                cp_async_arrive(&full[s]);
+            }
+            seq += n_kb;
+        }
+        if (!ok) give_up();
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else {
+        // ---------------------------------------------------------- epilogue
+        // Warps 4-7 and 8-11 take alternate 16-column chunks; within a chunk
+        // warp w of four reads tensor-memory lanes 32 w .. 32 w + 31.
+        constexpr int kChunks = NT / 32;  // chunks of one warp
+        const int w = (warp - 4) & 3, side = (warp - 4) >> 2;
+        float *xch = reinterpret_cast<float *>(sm + L::kOffXch);
+        int it = 0, parity = 0;
+        for (int t = blockIdx.x; t < total; t += gridDim.x, it++) {
+            const Tile q = find_tile<NT>(off, pre, a.n_group, n_mt, t);
+            const int b = it & 1;
+            // While the products run: where each column's row goes and its
+            // weight. Lane l looks up column l % 16 of every chunk.
+            int orow[kChunks];
+            float rw[kChunks];
+            uint32_t good = 0;  // bit j: chunk j's column has a valid token row
+#pragma unroll
+            for (int j = 0; j < kChunks; j++) {
+                const int c = 16 * (side + 2 * j) + (lane & 15), r = q.r0 + c;
+                const bool report = w == 0 && lane < 16;
+                orow[j] = -1;
+                rw[j] = 1.0f;
+                if (c >= q.rows) continue;
+                int xid = r;
+                bool ok_x = true;
+                if (GATHER) {
+                    xid = a.x_rows[r];
+                    ok_x = xid >= 0 && xid / a.x_div < a.n_x;
+                    if (!ok_x && report) flag_error(err, kErrBadId);
+                }
+                good |= (uint32_t)ok_x << j;
+                if (SWIGLU) {
+                    if (a.row_w && ok_x) rw[j] = a.row_w[xid];
+                } else {
+                    orow[j] = r;
+                    if (a.out_rows) {
+                        const int o = a.out_rows[r];
+                        orow[j] = o >= 0 && o < a.n_out_rows ? o : -1;
+                        if (orow[j] < 0 && report) flag_error(err, kErrBadId);
+                    }
+                }
+            }
+            // The warps go on together or not at all.
+            ok = named_all(3, kEpilogueThreads, mbar_wait(&acc_full[b], (it >> 1) & 1u, kWaitLimit));
+            if (!ok) {
+                give_up();
+                break;
+            }
+            tc_fence_after();
+            const uint32_t d = tmem + b * NT + ((uint32_t)(32 * w) << 16);
+#pragma unroll
+            for (int j = 0; j < kChunks; j++) {
+                const int c0 = 16 * (side + 2 * j), nc = min(16, q.rows - c0);
+                if (nc <= 0) break;
+                uint32_t v[16];
+                tc_ld16(v, d + c0);
+                const unsigned good_mask = __ballot_sync(kFull, (good >> j) & 1u);
+                if (SWIGLU) {
+                    // Warps 0 / 1 hold gate lanes, 2 / 3 the same up lanes. Of a
+                    // pair, the gate warp finishes the even columns and the up
+                    // warp the odd ones; each sends the other its half.
+                    const int me = side * 4 + w;
+                    float *mine = xch + (me * 2 + parity) * 256;
+                    const float *theirs = xch + ((me ^ 2) * 2 + parity) * 256;
+                    parity ^= 1;
+                    const bool gate = w < 2;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) mine[i * 32 + lane] = __uint_as_float(gate ? v[2 * i + 1] : v[2 * i]);
+                    named_sync(4 + side * 2 + (w & 1), 64);
+                    const int f0 = q.mt * kRowsPerTile + 32 * (w & 1);
+                    uint32_t my_scale = 0;
+                    uint8_t *oq = reinterpret_cast<uint8_t *>(a.out) + (size_t)(q.r0 + c0) * a.n_w + f0 + lane;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int c = 2 * i + (gate ? 0 : 1);
+                        if (c >= nc) break;
+                        const float other = theirs[i * 32 + lane];
+                        const float gv = gate ? __uint_as_float(v[2 * i]) : other;
+                        const float uv = gate ? other : __uint_as_float(v[2 * i + 1]);
+                        // silu(g) u: the quotient is good to 2 ulp, far inside the 8-bit rounding.
+                        float h = __fdividef(gv, 1.0f + expf(-gv)) * uv;
+                        if (a.row_w) h *= __shfl_sync(kFull, rw[j], c);
+                        if (!((good_mask >> c) & 1u)) h = 0.0f;
+                        const uint32_t amax = __reduce_max_sync(kFull, __float_as_uint(h) & 0x7fffffffu);
+                        const uint32_t sc = mx_scale<kMxEmaxFp8>(amax);
+                        const uint32_t e = e4m3x2(mx_scaled(h, sc, mx_inv_scale(sc)), 0.0f);
+                        if (lane == c) my_scale = sc;
+                        if (f0 < a.n_w) oq[(size_t)c * a.n_w] = (uint8_t)e;
+                    }
+                    if ((lane & 1) == (gate ? 0 : 1) && lane < nc && f0 < a.n_w)
+                        a.out_s[(size_t)(q.r0 + c0 + lane) * (a.n_w / kMxBlock) + f0 / kMxBlock] = (uint8_t)my_scale;
+                } else {
+                    const int m = q.mt * kRowsPerTile + 32 * w + lane;
+                    if (good_mask != kFull) {
+#pragma unroll
+                        for (int c = 0; c < 16; c++)
+                            if (!((good_mask >> c) & 1u)) v[c] = 0u;
+                    }
+                    if (a.half) {
+                        __half *o = reinterpret_cast<__half *>(a.out) + m;
+#pragma unroll
+                        for (int c = 0; c < 16; c++) {
+                            const int row = __shfl_sync(kFull, orow[j], c);
+                            if (row >= 0 && m < a.n_w) o[(size_t)row * a.n_w] = __float2half_rn(__uint_as_float(v[c]));
+                        }
+                    } else {
+                        float *o = reinterpret_cast<float *>(a.out) + m;
+#pragma unroll
+                        for (int c = 0; c < 16; c++) {
+                            const int row = __shfl_sync(kFull, orow[j], c);
+                            if (row >= 0 && m < a.n_w) o[(size_t)row * a.n_w] = __uint_as_float(v[c]);
+                        }
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[b]);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::kTmemCols) : "memory");
+}
+
+// ---------------------------------------------------------------- host side
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_fn()
+{
+    static EncodeTiled fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult st;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12080, cudaEnableDefault, &st) != cudaSuccess ||
+            st != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return (EncodeTiled)p;
+    }();
+    return fn;
+}
+
+// Rows of `cols` elements, `rows` per matrix, `n` matrices; 128 elements by
+// `box_rows` rows per copy, 128-byte swizzle. fp4: packed in memory, one byte
+// per element in shared memory.
+bool encode(CUtensorMap *m, const void *base, int rank, uint64_t cols, uint64_t rows, uint64_t n, uint32_t box_rows, bool fp4)
+{
+    const uint64_t row_bytes = fp4 ? cols / 2 : cols;
+    const cuuint64_t dim[3] = {cols, rows, n};
+    const cuuint64_t stride[2] = {row_bytes, row_bytes * rows};
+    const cuuint32_t box[3] = {kStageK, box_rows, 1};
+    const cuuint32_t step[3] = {1, 1, 1};
+    EncodeTiled fn = encode_fn();
+    return fn && fn(m, fp4 ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_UINT8, (cuuint32_t)rank,
+                    const_cast<void *>(base), dim, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int scale_vec(const void *base, int n)
+{
+    const uintptr_t v = (uintptr_t)base | (uintptr_t)n;
+    return v % 16 == 0 ? 16 : v % 8 == 0 ? 8 : v % 4 == 0 ? 4 : 1;
+}
+
+template <int NT, bool SWIGLU, bool GATHER>
+cudaError_t launch_nt(const LaunchCtx &c, const MoeMaps &maps, const MoeArgs &a)
+{
+    using L = MoeLayout<NT>;
+    auto *k = moe_mx_k<NT, SWIGLU, GATHER>;
+    static const cudaError_t set = [&] {
+        keep_driver_carveout((const void *)k);
+        return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kSmem);
+    }();
+    if (set != cudaSuccess) return set;
+    const int rows_per_tile = SWIGLU ? kTileM / 2 : kTileM;
+    const int64_t n_mt = (a.n_w + rows_per_tile - 1) / rows_per_tile;
+    const int64_t tiles = ((int64_t)a.n_rows / NT + (a.n_rows < a.n_group ? a.n_rows : a.n_group)) * n_mt;
+    if (tiles > 0x3fffffff) return cudaErrorInvalidValue;
+    const unsigned grid = (unsigned)(tiles < c.n_sm ? tiles : c.n_sm);
+    launch_ks(c, k, dim3(grid), dim3(moe_threads(GATHER)), L::kSmem, maps, a, c.err);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_moe_mx(const LaunchCtx &c, const MoeMxCall &q)
+{
+    if (q.n_rows <= 0 || q.n_group <= 0) return cudaSuccess;
+    if (q.n_group > kMaxGroups) return cudaErrorInvalidValue;
+    MoeMaps maps;
+    const bool fp4 = q.w_type == kMxFp4, swiglu = q.w1 != nullptr;
+    if (!encode(&maps.w0, q.w0, 3, q.K, q.n_w, q.n_group, swiglu ? kTileM / 2 : kTileM, fp4) ||
+        !encode(&maps.w1, swiglu ? q.w1 : q.w0, 3, q.K, q.n_w, q.n_group, kTileM / 2, fp4) ||
+        !encode(&maps.x, q.x, 2, q.K, q.n_x, 1, 32, false))
+        return cudaErrorInvalidValue;
+    const int nk32 = q.K / kMxBlock;
+    MoeArgs a = {};
+    a.x = q.x;
+    a.x_s = q.x_s;
+    a.half = q.out_f16;
+    a.fp4 = fp4;
+    a.w0_s = q.w0_s;
+    a.w1_s = q.w1_s;
+    a.offsets = q.offsets;
+    a.x_rows = q.x_rows;
+    a.row_w = q.row_w;
+    a.out_rows = q.out_rows;
+    a.out = q.out;
+    a.out_s = q.out_s;
+    a.n_x = q.n_x;
+    a.n_rows = q.n_rows;
+    a.n_out_rows = q.n_out_rows;
+    a.n_group = q.n_group;
+    a.x_div = q.x_div;
+    a.K = q.K;
+    a.n_w = q.n_w;
+    a.x_vec = scale_vec(q.x_s, nk32);
+    a.w_vec = swiglu ? min(scale_vec(q.w0_s, nk32), scale_vec(q.w1_s, nk32)) : scale_vec(q.w0_s, nk32);
+    const int avg = (q.n_rows + q.n_group - 1) / q.n_group;
+    const int nt = avg <= 64 ? 64 : avg <= 256 ? 128 : 224;
+#define DS3_MOE(NT)                                                                                       \
+    (swiglu ? (q.x_rows ? launch_nt<NT, true, true>(c, maps, a) : launch_nt<NT, true, false>(c, maps, a)) \
+            : (q.x_rows ? launch_nt<NT, false, true>(c, maps, a) : launch_nt<NT, false, false>(c, maps, a)))
+    return nt == 64 ? DS3_MOE(64) : nt == 128 ? DS3_MOE(128) : DS3_MOE(224);
+#undef DS3_MOE
+}
+
+}  // namespace ds3

@@ -104,6 +104,70 @@ __global__ void __launch_bounds__(kRouteThreads) moe_expert_lists_k(
     if (tid == 0) counts[ex] = (int32_t)(base < cap ? base : cap);
 }
 
+// Sorted rows without list capacities: entries (token * n_used + slot) in
+// expert order, each expert's in ascending order, and the experts' bounds.
+// One CTA per expert. Thread t owns a contiguous run of entries: it counts
+// those of smaller experts and of its own, one CTA-wide scan places its run,
+// and a second walk over the run (from L2) writes the hits out. offsets[ex] is
+// the number of entries of smaller experts, so no CTA waits for another.
+__global__ void __launch_bounds__(kRouteThreads) moe_expert_rows_k(const int32_t *idx, int32_t *offsets, int32_t *entries,
+                                                                   int32_t *row_of, int n_entries, int n_expert, int run,
+                                                                   int vec, unsigned *err)
+{
+    __shared__ int32_t wpre[kRouteWarps], wless[kRouteWarps];
+    pdl_wait();
+    pdl_trigger();
+    const int ex = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int lo = min(n_entries, tid * run), hi = min(n_entries, lo + run);  // run % 4 == 0
+    auto walk = [&](auto &&f) {
+        int i = lo;
+        if (vec) {
+#pragma unroll 4
+            for (; i + 4 <= hi; i += 4) {
+                const int4 e = *reinterpret_cast<const int4 *>(idx + i);
+                f(i, e.x);
+                f(i + 1, e.y);
+                f(i + 2, e.z);
+                f(i + 3, e.w);
+            }
+        }
+        for (; i < hi; i++) f(i, idx[i]);
+    };
+    int mine = 0, less = 0;
+    walk([&](int i, int e) {
+        mine += e == ex;
+        less += e >= 0 && e < ex;
+        if (ex == 0 && (e < 0 || e >= n_expert)) {
+            flag_error(err, kErrBadId);
+            if (row_of) row_of[i] = -1;
+        }
+    });
+    int inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(kFull, inc, o);
+        if (lane >= o) inc += y;
+    }
+    less = __reduce_add_sync(kFull, less);
+    if (lane == 31) wpre[warp] = inc;
+    if (lane == 0) wless[warp] = less;
+    __syncthreads();
+    const int in_warp = wpre[lane];
+    const int first = __reduce_add_sync(kFull, wless[lane]);               // entries of smaller experts
+    const int before = __reduce_add_sync(kFull, lane < warp ? in_warp : 0);  // this expert's, in earlier warps
+    int row = first + before + inc - mine;
+    if (mine)
+        walk([&](int i, int e) {
+            if (e != ex) return;
+            entries[row] = i;
+            if (row_of) row_of[i] = row;
+            row++;
+        });
+    if (tid == 0) offsets[ex] = first;
+    if (ex == n_expert - 1 && tid == kRouteThreads - 1) offsets[n_expert] = first + before + inc;
+}
+
 // Self-test of the bounded mbarrier wait: the barrier expects one arrival
 // that never comes; the wait must give up after `polls` polls and record the
 // timeout in the error word.
@@ -143,6 +207,17 @@ cudaError_t launch_moe_expert_lists(const LaunchCtx &c, const int32_t *idx, cons
     if (n_expert <= 0 || n_expert > 65535) return cudaErrorInvalidValue;
     launch_k(c, moe_expert_lists_k, dim3((unsigned)n_expert), dim3(kRouteThreads), idx, scores, counts, ids, gscores, slot_of,
              n_tokens * n_used, n_used, n_expert, cap, c.err);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_moe_expert_rows(const LaunchCtx &c, const int32_t *idx, int32_t *offsets, int32_t *entries,
+                                   int32_t *row_of, int64_t n_entries, int n_expert)
+{
+    if (n_expert <= 0 || n_expert > 65535 || n_entries > (1 << 30)) return cudaErrorInvalidValue;
+    const int run = (int)((n_entries + kRouteThreads - 1) / kRouteThreads + 3) & ~3;
+    const int vec = (reinterpret_cast<uintptr_t>(idx) & 15u) == 0;
+    launch_k(c, moe_expert_rows_k, dim3((unsigned)n_expert), dim3(kRouteThreads), idx, offsets, entries, row_of,
+             (int)n_entries, n_expert, run, vec, c.err);
     return cudaGetLastError();
 }
 

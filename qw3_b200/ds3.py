@@ -28,6 +28,9 @@ HEADERS = sorted((ROOT / "include").glob("*.h"))
 # ds3_type_t (src/ds3.h:201-216 of the reference)
 TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_Q4_K, TYPE_Q6_K = 0, 1, 8, 12, 14
 
+# ds3_cuda_mx_t
+MXFP8, MXFP4 = 0, 1
+
 TIMER_SLOTS = 16384
 
 _lib = None
@@ -82,6 +85,12 @@ _SIGS = {
     "moe_ffn_router_topk": (_I, [_P, _P, _U64, _I, _P, _P, _P, _U32, _U32, _U32, _U32, _B]),
     "moe_ffn_router_topk_noalloc": (_I, [_P, _P, _U64, _I, _P, _P, _P, _U32, _U32, _U32, _U32, _B]),
     "moe_combine_residual": (_I, [_P, _P, _P, _P, _P, _U32, _U32, _U32]),
+    "mx_quantize": (_I, [_P, _I, _P, _P, _I, _U64, _U32]),
+    "mx_dequantize": (_I, [_P, _P, _I, _P, _U64, _U32]),
+    "add_rms_norm_mx": (_I, [_P, _P, _P, _P, _P, _P, _P, _U32, _U32, _F]),
+    "moe_expert_rows": (_I, [_P, _P, _P, _P, _U32, _U32, _U32]),
+    "moe_mx_matmul": (_I, [_P, _P, _P, _U32, _P, _P, _P, _I, _P, _I, _P, _U32, _U32, _U32, _U32, _U32]),
+    "moe_mx_swiglu": (_I, [_P, _P, _P, _U32, _P, _P, _P, _P, _P, _I, _P, _P, _P, _U32, _U32, _U32, _U32, _U32]),
     "stream": (_P, []),
     "lane_write": (_I, [_I, _P, _SZ, _P, _SZ]),
     "lane_read": (_I, [_I, _P, _SZ, _P, _SZ]),
@@ -427,6 +436,37 @@ def swiglu(gate, up, row_weight, out, n_rows, n_cols) -> int:
 def moe_combine_residual(y, y_rows, w, residual, out, n_tokens, n_used, n_cols) -> int:
     return lib().ds3_cuda_moe_combine_residual(_h(y), _h(y_rows), _h(w), _h(residual), _h(out), n_tokens,
                                                n_used, n_cols)
+
+
+# ------------------------------------- microscaled rows, the experts' products
+def mx_quantize(src, src_type, q, scales, to, n_rows, n_cols) -> int:
+    return lib().ds3_cuda_mx_quantize(_h(src), src_type, _h(q), _h(scales), to, n_rows, n_cols)
+
+
+def mx_dequantize(q, scales, from_, dst, n_rows, n_cols) -> int:
+    return lib().ds3_cuda_mx_dequantize(_h(q), _h(scales), from_, _h(dst), n_rows, n_cols)
+
+
+def add_rms_norm_mx(x, residual, weight, sum_out, norm_out, q, scales, n, n_rows, eps) -> int:
+    return lib().ds3_cuda_add_rms_norm_mx(_h(x), _h(residual), _h(weight), _h(sum_out), _h(norm_out), _h(q), _h(scales),
+                                          n, n_rows, eps)
+
+
+def moe_expert_rows(idx, offsets, entries, row_of, n_tokens, n_expert, n_used) -> int:
+    return lib().ds3_cuda_moe_expert_rows(_h(idx), _h(offsets), _h(entries), _h(row_of), n_tokens, n_expert, n_used)
+
+
+def moe_mx_matmul(x_q, x_scales, x_rows, x_div, offsets, w_q, w_scales, w_type, out, out_type, out_rows, n_x, n_rows,
+                  n_expert, n_in, n_out) -> int:
+    return lib().ds3_cuda_moe_mx_matmul(_h(x_q), _h(x_scales), _h(x_rows), x_div, _h(offsets), _h(w_q), _h(w_scales),
+                                        w_type, _h(out), out_type, _h(out_rows), n_x, n_rows, n_expert, n_in, n_out)
+
+
+def moe_mx_swiglu(x_q, x_scales, x_rows, x_div, offsets, gate_q, gate_scales, up_q, up_scales, w_type, row_weight, act_q,
+                  act_scales, n_x, n_rows, n_expert, n_in, n_ff) -> int:
+    return lib().ds3_cuda_moe_mx_swiglu(_h(x_q), _h(x_scales), _h(x_rows), x_div, _h(offsets), _h(gate_q),
+                                        _h(gate_scales), _h(up_q), _h(up_scales), w_type, _h(row_weight), _h(act_q),
+                                        _h(act_scales), n_x, n_rows, n_expert, n_in, n_ff)
 
 
 # ------------------------------------------------- streams / graphs / timers
