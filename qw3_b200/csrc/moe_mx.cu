@@ -74,7 +74,8 @@ struct MoeLayout {
     static constexpr int kOffXch = kOffSfB + kStages * kSfB;
     static constexpr int kOffTab = kOffXch + kXch;        // first row, rows and first tile of each group
     static constexpr int kOffIds = kOffTab + 3 * kMaxGroups * 4;  // gathered row ids, per gathering warp
-    static constexpr int kUsed = kOffIds + 4 * NT * 4;
+    static constexpr int kOffCol = kOffIds + 4 * NT * 4;                // epilogue columns, two tiles
+    static constexpr int kUsed = kOffCol + 2 * NT * 8;
     static constexpr size_t kSmem = kUsed + 1024;         // the base is aligned up to 1024
     static constexpr int kSfCols = 4 + kBWords;
     static constexpr int kColsUsed = 2 * NT + kStages * kSfCols;
@@ -103,17 +104,30 @@ struct MoeArgs {
 };
 
 // ------------------------------------------------------------ PTX wrappers
-__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *m, int x, int y, int z, uint64_t *bar)
+// The single-thread instructions below are executed by whole warps and
+// predicated on `lead` (one lane's flag): control flow stays uniform, so their
+// operands are computed once in uniform registers. Branching into one lane
+// instead cost about twice the issue time per stage.
+__device__ __forceinline__ void tma_load_3d(uint32_t lead, uint32_t dst, const CUtensorMap *m, int x, int y, int z,
+                                            uint32_t bar)
 {
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
-            "r"(smem_addr(dst)), "l"(m), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar)) : "memory");
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "@q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n\t}" ::
+            "r"(dst), "l"(m), "r"(x), "r"(y), "r"(z), "r"(bar), "r"(lead) : "memory");
 }
-__device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *m, int x, int y, uint64_t *bar)
+__device__ __forceinline__ void tma_load_2d(uint32_t lead, uint32_t dst, const CUtensorMap *m, int x, int y, uint32_t bar)
 {
     asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
-            "r"(smem_addr(dst)), "l"(m), "r"(x), "r"(y), "r"(smem_addr(bar)) : "memory");
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n\t}" ::
+            "r"(dst), "l"(m), "r"(x), "r"(y), "r"(bar), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void expect_bytes(uint32_t lead, uint32_t bar, uint32_t bytes)
+{
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+        "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes), "r"(lead) : "memory");
 }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src)
 {
@@ -136,24 +150,28 @@ __device__ __forceinline__ bool elect_one()
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// Arrive on `bar` once all tensor-core work this thread issued has finished.
-__device__ __forceinline__ void tc_commit(uint64_t *bar)
+// Arrive on `bar` once all tensor-core work the lead lane issued has finished.
+__device__ __forceinline__ void tc_commit(uint32_t lead, uint32_t bar)
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
-                 : "memory");
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(lead)
+        : "memory");
 }
 // 32 rows of 16 bytes, shared -> tensor memory, into all four lane quarters.
-__device__ __forceinline__ void tc_copy_scales(uint32_t tmem, uint64_t desc)
+__device__ __forceinline__ void tc_copy_scales(uint32_t lead, uint32_t tmem, uint64_t desc)
 {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+        "@q tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(tmem), "l"(desc), "r"(lead) : "memory");
 }
-__device__ __forceinline__ void tc_mma_mx(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,
+__device__ __forceinline__ void tc_mma_mx(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,
                                           uint32_t sfb, uint32_t accumulate)
 {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::
-            "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 q, %7, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::
+            "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(lead) : "memory");
 }
 __device__ __forceinline__ void tc_ld16(uint32_t (&v)[16], uint32_t tmem)
 {
@@ -349,50 +367,45 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
 
     if (warp == 0) {
         // ------------------------------------------------------------ copies
-        // One thread runs the stages of a tile: per stage a wait, the byte
-        // count and the copies, without warp votes in between.
+        const uint32_t lead = elect_one();
+        const uint32_t full0 = smem_addr(&full[0]), a0 = smem_addr(sm + L::kOffA), b0 = smem_addr(sm + L::kOffB);
         int s = 0, issued = 0;
         uint32_t ph = 0;
-        for (int t = blockIdx.x; t < total; t += gridDim.x) {
+        for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
             const Tile q = find_tile<NT>(tab, a, t, lane);
-            if (elect_one()) {
-                const int nbox = GATHER ? 0 : (q.rows + 31) >> 5;
-                const uint32_t bytes = (a.fp4 ? L::kABytes / 2 : L::kABytes) + nbox * 4096;
-                const int row = q.mt * kRowsPerTile;
-                int u = s;
-                uint32_t p = ph;
-                for (int kb = 0; kb < n_kb; kb++) {
-                    ok = mbar_wait(&empty[u], p ^ 1u, kWaitLimit);
-                    if (!ok) break;
-                    uint8_t *A = sm + L::kOffA + u * L::kABytes, *B = sm + L::kOffB + u * L::kBBytes;
-                    mbar_expect_tx(&full[u], bytes);
-                    tma_load_3d(A, &maps.w0, kb * kStageK, row, q.e, &full[u]);
-                    if (SWIGLU) tma_load_3d(A + L::kABytes / 2, &maps.w1, kb * kStageK, row, q.e, &full[u]);
-                    if (!GATHER)
-                        for (int i = 0; i < nbox; i++)
-                            tma_load_2d(B + i * 4096, &maps.x, kb * kStageK, q.r0 + 32 * i, &full[u]);
-                    issued++;
-                    if (++u == ST) {
-                        u = 0;
-                        p ^= 1u;
-                    }
-                }
-                if (!ok) {
-                    give_up();
-                    // Let the copies in flight land before shared memory goes away.
-                    for (int i = 0; i < ST && i < issued; i++) {
-                        if (u == 0) p ^= 1u;
-                        u = u == 0 ? ST - 1 : u - 1;
-                        mbar_wait(&full[u], p, kWaitLimit);
-                    }
+            const int nbox = GATHER ? 0 : (q.rows + 31) >> 5;
+            const uint32_t bytes = (a.fp4 ? L::kABytes / 2 : L::kABytes) + nbox * 4096;
+            const int row = q.mt * kRowsPerTile;
+            for (int kb = 0; kb < n_kb; kb++) {
+                ok = __all_sync(kFull, mbar_wait(&empty[s], ph ^ 1u, kWaitLimit));
+                if (!ok) break;
+                const uint32_t bar = full0 + 8 * s, A = a0 + s * L::kABytes, B = b0 + s * L::kBBytes;
+                expect_bytes(lead, bar, bytes);
+                tma_load_3d(lead, A, &maps.w0, kb * kStageK, row, q.e, bar);
+                if (SWIGLU) tma_load_3d(lead, A + L::kABytes / 2, &maps.w1, kb * kStageK, row, q.e, bar);
+                if (!GATHER)
+                    for (int i = 0; i < nbox; i++)
+                        tma_load_2d(lead, B + i * 4096, &maps.x, kb * kStageK, q.r0 + 32 * i, bar);
+                issued++;
+                if (++s == ST) {
+                    s = 0;
+                    ph ^= 1u;
                 }
             }
-            if (!__all_sync(kFull, ok)) break;
-            ph ^= (uint32_t)((s + n_kb) / ST) & 1u;
-            s = (s + n_kb) % ST;
+        }
+        if (!ok) {
+            give_up();
+            // Let the copies in flight land before shared memory goes away.
+            for (int i = 0; i < ST && i < issued; i++) {
+                if (s == 0) ph ^= 1u;
+                s = s == 0 ? ST - 1 : s - 1;
+                mbar_wait(&full[s], ph, kWaitLimit);
+            }
         }
     } else if (warp == 1) {
         // ------------------------------------------------------ tensor cores
+        const uint32_t lead = elect_one();
+        const uint32_t empty0 = smem_addr(&empty[0]);
         int s = 0, it = 0;
         uint32_t ph = 0;
         // A's type (5 = e2m1, 0 = e4m3), power-of-two scales, M.
@@ -405,46 +418,40 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
         for (int t = blockIdx.x; t < total; t += gridDim.x, it++) {
             const Tile q = find_tile<NT>(tab, a, t, lane);
             const int b = it & 1;
-            if (elect_one()) {
-                ok = mbar_wait(&acc_empty[b], ((it >> 1) & 1u) ^ 1u, kWaitLimit);
+            ok = __all_sync(kFull, mbar_wait(&acc_empty[b], ((it >> 1) & 1u) ^ 1u, kWaitLimit));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t idesc = idesc0 | ((uint32_t)((q.rows + 15) >> 4) << 18);  // N / 8 at bit 17
+            const uint32_t d = tmem + b * NT;
+            for (int kb = 0; kb < n_kb; kb++) {
+                ok = __all_sync(kFull, mbar_wait(&full[s], ph, kWaitLimit));
+                if (!ok) break;
                 tc_fence_after();
-                const uint32_t idesc = idesc0 | ((uint32_t)((q.rows + 15) >> 4) << 18);  // N / 8 at bit 17
-                const uint32_t d = tmem + b * NT;
-                int u = s;
-                uint32_t p = ph;
-                for (int kb = 0; ok && kb < n_kb; kb++) {
-                    ok = mbar_wait(&full[u], p, kWaitLimit);
-                    if (!ok) break;
-                    tc_fence_after();
-                    fence_async_shared();
-                    const uint32_t sfa = tmem + 2 * NT + u * L::kSfCols, sfb = sfa + 4;
-                    tc_copy_scales(sfa, sa0 + u * (L::kSfA >> 4));
+                fence_async_shared();
+                const uint32_t sfa = tmem + 2 * NT + s * L::kSfCols, sfb = sfa + 4;
+                tc_copy_scales(lead, sfa, sa0 + s * (L::kSfA >> 4));
 #pragma unroll
-                    for (int j = 0; j < L::kBWords / 4; j++)
-                        tc_copy_scales(sfb + 4 * j, sb0 + u * (L::kSfB >> 4) + j * 32);
-                    const uint64_t ad = ad0 + u * (L::kABytes >> 4), bd = bd0 + u * (L::kBBytes >> 4);
-                    const int nk = nk32 - 4 * kb;  // 32-element steps left
+                for (int j = 0; j < L::kBWords / 4; j++)
+                    tc_copy_scales(lead, sfb + 4 * j, sb0 + s * (L::kSfB >> 4) + j * 32);
+                const uint64_t ad = ad0 + s * (L::kABytes >> 4), bd = bd0 + s * (L::kBBytes >> 4);
+                const int nk = nk32 - 4 * kb;  // 32-element steps left
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (i < nk)
-                            tc_mma_mx(d, ad + 2 * i, bd + 2 * i, idesc + i * kNextScale, sfa, sfb, (uint32_t)(kb | i));
-                    tc_commit(&empty[u]);
-                    if (++u == ST) {
-                        u = 0;
-                        p ^= 1u;
-                    }
-                }
-                if (ok) {
-                    tc_commit(&acc_full[b]);
-                } else {
-                    give_up();
-                    tc_commit(&drain);  // products in flight finish before tensor memory is freed
-                    mbar_wait(&drain, 0, kWaitLimit);
+                for (int i = 0; i < 4; i++)
+                    if (i < nk)
+                        tc_mma_mx(lead, d, ad + 2 * i, bd + 2 * i, idesc + i * kNextScale, sfa, sfb, (uint32_t)(kb | i));
+                tc_commit(lead, empty0 + 8 * s);
+                if (++s == ST) {
+                    s = 0;
+                    ph ^= 1u;
                 }
             }
-            if (!__all_sync(kFull, ok)) break;
-            ph ^= (uint32_t)((s + n_kb) / ST) & 1u;
-            s = (s + n_kb) % ST;
+            if (!ok) break;
+            tc_commit(lead, smem_addr(&acc_full[b]));
+        }
+        if (!ok) {
+            give_up();
+            tc_commit(lead, smem_addr(&drain));  // products in flight finish before tensor memory is freed
+            mbar_wait(&drain, 0, kWaitLimit);
         }
     } else if (warp < 4) {
         // ------------------------------------------------------------ scales
@@ -523,43 +530,37 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
         // ---------------------------------------------------------- epilogue
         // Warps 4-7 and 8-11 take alternate 16-column chunks; within a chunk
         // warp w of four reads tensor-memory lanes 32 w .. 32 w + 31.
-        constexpr int kChunks = NT / 32;  // chunks of one warp
-        const int w = (warp - 4) & 3, side = (warp - 4) >> 2;
+        const int w = (warp - 4) & 3, side = (warp - 4) >> 2, me = tid - 128;
+        static_assert(NT <= kEpilogueThreads, "one column per epilogue thread");
         float *xch = reinterpret_cast<float *>(sm + L::kOffXch);
         int it = 0, parity = 0;
         for (int t = blockIdx.x; t < total; t += gridDim.x, it++) {
             const Tile q = find_tile<NT>(tab, a, t, lane);
             const int b = it & 1;
-            // While the products run: where each column's row goes and its
-            // weight. Lane l looks up column l % 16 of every chunk.
-            int orow[kChunks];
-            float rw[kChunks];
-            uint32_t good = 0;  // bit j: chunk j's column has a valid token row
-#pragma unroll
-            for (int j = 0; j < kChunks; j++) {
-                const int c = 16 * (side + 2 * j) + (lane & 15), r = q.r0 + c;
-                const bool report = w == 0 && lane < 16;
-                orow[j] = -1;
-                rw[j] = 1.0f;
-                if (c >= q.rows) continue;
+            // While the products run, thread c looks up column c: where its row
+            // goes (-1: nowhere; SwiGLU: its weight) and whether its token row
+            // is one of x. Two buffers: no thread is two tiles ahead of another.
+            int2 *col = reinterpret_cast<int2 *>(sm + L::kOffCol) + b * NT;
+            if (me < q.rows) {
+                const int r = q.r0 + me;
                 int xid = r;
-                bool ok_x = true;
+                bool good = true;
                 if (GATHER) {
                     xid = a.x_rows[r];
-                    ok_x = xid >= 0 && xid / a.x_div < a.n_x;
-                    if (!ok_x && report) flag_error(err, kErrBadId);
+                    good = xid >= 0 && xid / a.x_div < a.n_x;
+                    if (!good) flag_error(err, kErrBadId);
                 }
-                good |= (uint32_t)ok_x << j;
+                int to = r;
                 if (SWIGLU) {
-                    if (a.row_w && ok_x) rw[j] = a.row_w[xid];
-                } else {
-                    orow[j] = r;
-                    if (a.out_rows) {
-                        const int o = a.out_rows[r];
-                        orow[j] = o >= 0 && o < a.n_out_rows ? o : -1;
-                        if (orow[j] < 0 && report) flag_error(err, kErrBadId);
+                    to = __float_as_int(a.row_w && good ? a.row_w[xid] : 1.0f);
+                } else if (a.out_rows) {
+                    to = a.out_rows[r];
+                    if (to < 0 || to >= a.n_out_rows) {
+                        to = -1;
+                        flag_error(err, kErrBadId);
                     }
                 }
+                col[me] = make_int2(to, good);
             }
             // The warps go on together or not at all.
             ok = named_all(3, kEpilogueThreads, mbar_wait(&acc_full[b], (it >> 1) & 1u, kWaitLimit));
@@ -569,20 +570,20 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
             }
             tc_fence_after();
             const uint32_t d = tmem + b * NT + ((uint32_t)(32 * w) << 16);
-#pragma unroll
-            for (int j = 0; j < kChunks; j++) {
-                const int c0 = 16 * (side + 2 * j), nc = min(16, q.rows - c0);
-                if (nc <= 0) break;
+            // One copy of the chunk's code: with it unrolled over the chunks, the
+            // roles' instructions no longer fit the instruction caches together.
+#pragma unroll 1
+            for (int c0 = 16 * side; c0 < q.rows; c0 += 32) {
+                const int nc = min(16, q.rows - c0);
                 uint32_t v[16];
                 tc_ld16(v, d + c0);
-                const unsigned good_mask = __ballot_sync(kFull, (good >> j) & 1u);
                 if (SWIGLU) {
                     // Warps 0 / 1 hold gate lanes, 2 / 3 the same up lanes. Of a
                     // pair, the gate warp finishes the even columns and the up
                     // warp the odd ones; each sends the other its half.
-                    const int me = side * 4 + w;
-                    float *mine = xch + (me * 2 + parity) * 256;
-                    const float *theirs = xch + ((me ^ 2) * 2 + parity) * 256;
+                    const int at = side * 4 + w;
+                    float *mine = xch + (at * 2 + parity) * 256;
+                    const float *theirs = xch + ((at ^ 2) * 2 + parity) * 256;
                     parity ^= 1;
                     const bool gate = w < 2;
 #pragma unroll
@@ -598,10 +599,11 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
                         const float other = theirs[i * 32 + lane];
                         const float gv = gate ? __uint_as_float(v[2 * i]) : other;
                         const float uv = gate ? other : __uint_as_float(v[2 * i + 1]);
+                        const int2 k = col[c0 + c];
                         // silu(g) u: the quotient is good to 2 ulp, far inside the 8-bit rounding.
                         float h = __fdividef(gv, 1.0f + expf(-gv)) * uv;
-                        if (a.row_w) h *= __shfl_sync(kFull, rw[j], c);
-                        if (!((good_mask >> c) & 1u)) h = 0.0f;
+                        if (a.row_w) h *= __int_as_float(k.x);
+                        if (!k.y) h = 0.0f;
                         const uint32_t amax = __reduce_max_sync(kFull, __float_as_uint(h) & 0x7fffffffu);
                         const uint32_t sc = mx_scale<kMxEmaxFp8>(amax);
                         const uint32_t e = e4m3x2(mx_scaled(h, sc, mx_inv_scale(sc)), 0.0f);
@@ -612,24 +614,24 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
                         a.out_s[(size_t)(q.r0 + c0 + lane) * (a.n_w / kMxBlock) + f0 / kMxBlock] = (uint8_t)my_scale;
                 } else {
                     const int m = q.mt * kRowsPerTile + 32 * w + lane;
-                    if (good_mask != kFull) {
-#pragma unroll
-                        for (int c = 0; c < 16; c++)
-                            if (!((good_mask >> c) & 1u)) v[c] = 0u;
-                    }
+                    const bool in = m < a.n_w;
                     if (a.half) {
                         __half *o = reinterpret_cast<__half *>(a.out) + m;
 #pragma unroll
                         for (int c = 0; c < 16; c++) {
-                            const int row = __shfl_sync(kFull, orow[j], c);
-                            if (row >= 0 && m < a.n_w) o[(size_t)row * a.n_w] = __float2half_rn(__uint_as_float(v[c]));
+                            if (c >= nc) break;
+                            const int2 k = col[c0 + c];
+                            if (k.x >= 0 && in)
+                                o[(size_t)(uint32_t)k.x * (uint32_t)a.n_w] = __float2half_rn(k.y ? __uint_as_float(v[c]) : 0.0f);
                         }
                     } else {
                         float *o = reinterpret_cast<float *>(a.out) + m;
 #pragma unroll
                         for (int c = 0; c < 16; c++) {
-                            const int row = __shfl_sync(kFull, orow[j], c);
-                            if (row >= 0 && m < a.n_w) o[(size_t)row * a.n_w] = __uint_as_float(v[c]);
+                            if (c >= nc) break;
+                            const int2 k = col[c0 + c];
+                            if (k.x >= 0 && in)
+                                o[(size_t)(uint32_t)k.x * (uint32_t)a.n_w] = k.y ? __uint_as_float(v[c]) : 0.0f;
                         }
                     }
                 }
