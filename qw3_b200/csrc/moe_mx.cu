@@ -22,7 +22,7 @@
 // so the CTAs working at the same time share token rows and, with several
 // token blocks, weights through L2. The tile list is derived on the device
 // from `offsets`; the host never reads it.
-//   - 128 K elements per stage: A 16 KB, B NT x 128 B, both in the 128-byte
+//   - Slices of 128 K elements: A 16 KB, B NT x 128 B, both in the 128-byte
 //     swizzle, one 32-bit word of four scales per row.
 //   - tcgen05.mma kind::mxf8f6f4 with block scales, K = 32 per instruction,
 //     accumulators fp32 in tensor memory, double buffered so the epilogue of
@@ -53,31 +53,35 @@ namespace ds3 {
 namespace {
 
 constexpr int kTileM = 128;     // weight rows per tile
-constexpr int kStageK = 128;    // K elements per stage
+constexpr int kSliceK = 128;    // K elements per slice of a stage
 constexpr int kEpilogueThreads = 256, kGatherThreads = 128;
 constexpr int moe_threads(bool gather) { return 128 + kEpilogueThreads + (gather ? kGatherThreads : 0); }
 constexpr int kMaxGroups = 256;
 
-// Stages for NT token columns, as many as fit beside the exchange buffers.
+// Stages for NT token columns, as many as fit beside the exchange buffers. A
+// stage is kSub slices of 128 K elements: two where the slices are small, so
+// that the fixed work per stage (wait, fence, commit) of the issuing warp,
+// which bounds these sizes, is paid half as often.
 template <int NT>
 struct MoeLayout {
-    static constexpr int kStages = NT == 64 ? 8 : NT == 128 ? 6 : 4;
-    static constexpr int kABytes = kTileM * kStageK;
-    static constexpr int kBBytes = NT * kStageK;
-    static constexpr int kBWords = (NT + 127) / 128 * 4;  // tensor-memory columns of B's scales
-    static constexpr int kSfA = 512, kSfB = kBWords * 128;
+    static constexpr int kSub = NT <= 128 ? 2 : 1;
+    static constexpr int kStages = NT == 64 ? 4 : NT == 128 ? 3 : 4;
+    static constexpr int kASlice = kTileM * kSliceK, kBSlice = NT * kSliceK;
+    static constexpr int kABytes = kSub * kASlice, kBBytes = kSub * kBSlice;
+    static constexpr int kBWords = (NT + 127) / 128 * 4;  // tensor-memory columns of B's scales per slice
+    static constexpr int kSfA = kSub * 512, kSfB = kSub * kBWords * 128;
     static constexpr int kXch = 8 * 2 * 8 * 32 * 4;       // [epilogue warp][buffer][8][32] floats
     static constexpr int kOffA = 0;
     static constexpr int kOffB = kOffA + kStages * kABytes;
     static constexpr int kOffSfA = kOffB + kStages * kBBytes;
     static constexpr int kOffSfB = kOffSfA + kStages * kSfA;
     static constexpr int kOffXch = kOffSfB + kStages * kSfB;
-    static constexpr int kOffTab = kOffXch + kXch;        // first row, rows and first tile of each group
-    static constexpr int kOffIds = kOffTab + 3 * kMaxGroups * 4;  // gathered row ids, per gathering warp
-    static constexpr int kOffCol = kOffIds + 4 * NT * 4;                // epilogue columns, two tiles
+    static constexpr int kOffTab = kOffXch + kXch;        // first row, rows, first tile and block size of each group
+    static constexpr int kOffIds = kOffTab + 4 * kMaxGroups * 4;  // gathered row ids, per gathering warp
+    static constexpr int kOffCol = kOffIds + NT * 4;                    // epilogue columns, two tiles
     static constexpr int kUsed = kOffCol + 2 * NT * 8;
     static constexpr size_t kSmem = kUsed + 1024;         // the base is aligned up to 1024
-    static constexpr int kSfCols = 4 + kBWords;
+    static constexpr int kSfCols = kSub * (4 + kBWords);
     static constexpr int kColsUsed = 2 * NT + kStages * kSfCols;
     static constexpr int kTmemCols = kColsUsed <= 256 ? 256 : 512;
     static_assert(kColsUsed <= 512 && kSmem <= 232448 - 512, "layout");
@@ -98,7 +102,7 @@ struct MoeArgs {
     void *out;                 // fp32 / fp16 [n_out_rows][n_w], or e4m3 [n_rows][n_w]
     uint8_t *out_s;            // SwiGLU: [n_rows][n_w/32]
     int n_x, n_rows, n_out_rows, n_group, x_div, K, n_w;
-    int x_words, w_words;      // scale rows are whole aligned words
+    int x_mode, w_mode;        // how scale rows are loaded (stage_scales)
     unsigned n_mt, n_mt_inv;   // weight blocks per group, 2^32 / n_mt rounded up
     int half, fp4;             // out is fp16; the weights are MXFP4
 };
@@ -133,15 +137,46 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src)
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void *src)
-{
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
 // Arrive on `bar` once this thread's earlier cp.async copies have landed.
 __device__ __forceinline__ void cp_async_arrive(uint64_t *bar)
 {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
+// Whether the phase is complete now (no waiting).
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity)
+{
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done) : "r"(smem_addr(bar)), "r"(parity) : "memory");
+    return done != 0;
+}
+// A warp's place in the ring of stages. `ready` is a test of the next stage's
+// barrier made ahead of time: its latency (about 170 cycles with the vote)
+// passes under the work on the stage before.
+template <int ST>
+struct Ring {
+    int s = 0;
+    uint32_t ph;
+    bool ready = false;
+    __device__ __forceinline__ explicit Ring(uint32_t first) : ph(first) {}
+    __device__ __forceinline__ bool wait(uint64_t *bars)
+    {
+        return __all_sync(kFull, ready) || __all_sync(kFull, mbar_wait(&bars[s], ph, kWaitLimit));
+    }
+    // Test the stage after this one.
+    __device__ __forceinline__ void peek(uint64_t *bars)
+    {
+        ready = s + 1 == ST ? mbar_test(&bars[0], ph ^ 1u) : mbar_test(&bars[s + 1], ph);
+    }
+    __device__ __forceinline__ void next()
+    {
+        if (++s == ST) {
+            s = 0;
+            ph ^= 1u;
+        }
+    }
+};
 __device__ __forceinline__ bool elect_one()
 {
     uint32_t p;
@@ -212,6 +247,14 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t stride_byt
            (sw << 61);
 }
 
+// The row of x that an x_rows value names; one outside x reads row 0 (the
+// epilogue writes zeros for it).
+__device__ __forceinline__ int x_row(int v, const MoeArgs &a)
+{
+    const int x = v < 0 ? -1 : v / a.x_div;
+    return x < 0 || x >= a.n_x ? 0 : x;
+}
+
 struct Tile {
     int e, mt, n0, rows, r0;  // group, weight block, first row in the group, rows here, first sorted row
 };
@@ -222,7 +265,7 @@ struct Tile {
 template <int NT>
 __device__ __forceinline__ Tile find_tile(const int *tab, const MoeArgs &a, int t, int lane)
 {
-    const int *off = tab, *num = tab + kMaxGroups, *pre = tab + 2 * kMaxGroups;
+    const int *off = tab, *num = tab + kMaxGroups, *pre = tab + 2 * kMaxGroups, *size = tab + 3 * kMaxGroups;
     const int g = __popc(__ballot_sync(kFull, pre[8 * lane] <= t)) - 1;
     const int e = 8 * g + __popc(__ballot_sync(kFull, lane < 8 && pre[8 * g + (lane & 7)] <= t)) - 1;
     const unsigned local = t - pre[e];
@@ -232,56 +275,94 @@ __device__ __forceinline__ Tile find_tile(const int *tab, const MoeArgs &a, int 
     Tile q;
     q.e = e;
     q.mt = local - nt * a.n_mt;
-    q.n0 = nt * NT;
-    q.rows = min(num[e] - q.n0, NT);
+    q.n0 = nt * size[e];
+    q.rows = min(num[e] - q.n0, size[e]);
     q.r0 = off[e] + q.n0;
     return q;
 }
 
 // One warp stages the scales of J x 32 operand rows for every stage of every
 // tile of this CTA. Lane l owns rows l, l + 32, ...; the four scales of a row
-// and stage are one word, and the words of the lane's rows lie side by side,
-// which is the tensor core's order. Aligned rows (words) are copied
-// asynchronously, straight to their place: the ring of stages hides the
-// latency, where loads through registers had cost a memory round trip per 4
-// stages (512 tokens, 768 -> 2048: 61 us against 36 us without any loads).
-// Other rows (a K that is not a multiple of 128, an odd base) are put together
-// from bytes.
-template <int J, int BYTES, int ST, typename Rows>
-__device__ __forceinline__ bool stage_scales(Rows rows_of, uint8_t *dst, uint64_t *full, uint64_t *empty, int total,
-                                             int n_kb, int nk32, bool words, int lane)
+// and slice are one word, and the words of the lane's rows lie side by side,
+// which is the tensor core's order. They are loaded kAhead stages ahead of
+// their use in registers: MODE 2, all words of a row and stage at once (K a
+// whole number of stages); 1, word by word (K % 128 == 0); 0, words put
+// together from bytes (other K, an odd base).
+// Copying each word asynchronously to its place instead cost 52 cycles of
+// issue per copy and bounded the small tiles (512 tokens, 768 -> 2048: 33 us).
+constexpr int kAhead = 3;
+
+__device__ __forceinline__ void ld_word(uint32_t &v, const uint8_t *p)
 {
-    const uint8_t *row[J], *nxt[J];
-    int s = 0;
-    uint32_t ph = 0;
-    if (blockIdx.x < (unsigned)total) rows_of(row, blockIdx.x);
-    for (int t = blockIdx.x; t < total; t += gridDim.x) {
-        if (t + (int)gridDim.x < total) rows_of(nxt, t + gridDim.x);
-        for (int kb = 0; kb < n_kb; kb++) {
-            if (!__all_sync(kFull, mbar_wait(&empty[s], ph ^ 1u, kWaitLimit))) return false;
-            const uint32_t to = smem_addr(dst + s * BYTES) + lane * 16;
+    asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p));
+}
+__device__ __forceinline__ void ld_word2(uint32_t &v, uint32_t &w, const uint8_t *p)
+{
+    asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(v), "=r"(w) : "l"(p));
+}
+
+template <int J, int BYTES, int SUB, int ST, int MODE, typename Rows>
+__device__ __forceinline__ bool stage_scales(Rows &rows_of, uint8_t *dst, uint64_t *full, uint64_t *empty, int total,
+                                             int n_kb, int nk32, int lane)
+{
+    const uint8_t *row[J];
+    uint32_t buf[kAhead + 1][J][SUB];
+    int lt = blockIdx.x, lkb = 0;  // load cursor: tile, stage
+    auto load = [&](uint32_t (&v)[J][SUB]) {
+        if (lt >= total) return;
+        if (lkb == 0) rows_of(row, lt);
+        const int k = 4 * SUB * lkb;  // first scale of the stage
 #pragma unroll
-            for (int j = 0; j < J; j++) {
-                const uint32_t at = to + (j >> 2) * 512 + (j & 3) * 4;
-                if (words) {
-                    cp_async4(at, row[j] + 4 * kb);
-                } else {
-                    uint32_t v = 0;
+        for (int j = 0; j < J; j++) {
+            if (MODE == 2 && SUB == 2) {
+                ld_word2(v[j][0], v[j][SUB - 1], row[j] + k);
+            } else if (MODE) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (4 * kb + i < nk32) v |= (uint32_t)row[j][4 * kb + i] << (8 * i);
-                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+                for (int i = 0; i < SUB; i++)
+                    if (k + 4 * i < nk32) ld_word(v[j][i], row[j] + k + 4 * i);
+            } else {
+#pragma unroll
+                for (int i = 0; i < SUB; i++) {
+                    v[j][i] = 0;
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        if (k + 4 * i + c < nk32) v[j][i] |= (uint32_t)row[j][k + 4 * i + c] << (8 * c);
                 }
             }
-            if (words) cp_async_arrive(&full[s]);
-            else mbar_arrive(&full[s]);
-            if (++s == ST) {
-                s = 0;
-                ph ^= 1u;
+        }
+        if (++lkb == n_kb) {
+            lkb = 0;
+            lt += gridDim.x;
+        }
+    };
+    Ring<ST> ring(1u);
+    int t = blockIdx.x, kb = 0;
+#pragma unroll
+    for (int u = 0; u < kAhead; u++) load(buf[u]);
+    while (t < total) {
+#pragma unroll
+        for (int u = 0; u <= kAhead; u++) {
+            load(buf[(u + kAhead) % (kAhead + 1)]);
+            if (t < total) {
+                if (!ring.wait(empty)) return false;
+                ring.peek(empty);
+#pragma unroll
+                for (int i = 0; i < SUB; i++)
+#pragma unroll
+                    for (int j = 0; j < J; j += 4) {
+                        auto w = [&](int n) { return j + n < J ? buf[u][j + n < J ? j + n : 0][i] : 0u; };
+                        *reinterpret_cast<uint4 *>(dst + ring.s * BYTES + i * (BYTES / SUB) + j * 128 + lane * 16) =
+                            make_uint4(w(0), w(1), w(2), w(3));
+                    }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[ring.s]);
+                ring.next();
+                if (++kb == n_kb) {
+                    kb = 0;
+                    t += gridDim.x;
+                }
             }
         }
-#pragma unroll
-        for (int j = 0; j < J; j++) row[j] = nxt[j];
     }
     return true;
 }
@@ -307,8 +388,8 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int s = 0; s < ST; s++) {
-            // the copy thread and each lane of two scale warps and a gathering one
-            mbar_init(&full[s], 1 + 64 + (GATHER ? 32 : 0));
+            // the copy thread, the two scale warps and each gathering lane
+            mbar_init(&full[s], 3 + (GATHER ? kGatherThreads : 0));
             mbar_init(&empty[s], 1);
         }
         for (int b = 0; b < 2; b++) {
@@ -336,7 +417,10 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
             hi = min(max(h0, lo), a.n_rows);
             if ((lo != l0 || hi != h0) && blockIdx.x == 0) flag_error(err, kErrBadId);
         }
-        const int v = (hi - lo + NT - 1) / NT * (int)a.n_mt;
+        // A group's token blocks are of one size, a multiple of 16 (at most NT,
+        // so that the last one is never empty).
+        const int blocks = (hi - lo + NT - 1) / NT;
+        const int v = blocks * (int)a.n_mt;
         int inc = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -352,6 +436,7 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
             tab[tid] = lo;
             tab[kMaxGroups + tid] = hi - lo;
             tab[2 * kMaxGroups + tid] = base + inc - v;
+            tab[3 * kMaxGroups + tid] = blocks ? ((hi - lo + blocks - 1) / blocks + 15) & ~15 : NT;
         }
         if (tid == kMaxGroups - 1) n_tiles = base + inc;
     }
@@ -360,7 +445,8 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
     tc_fence_after();
     const int total = n_tiles;
     const uint32_t tmem = tmem_base;
-    const int n_kb = (a.K + kStageK - 1) / kStageK;
+    const int n_kb = (a.K + kSliceK * L::kSub - 1) / (kSliceK * L::kSub);  // stages per tile
+    const int n_slices = (a.K + kSliceK - 1) / kSliceK;
     const int nk32 = a.K / kMxBlock;
     bool ok = true;
     auto give_up = [&] { flag_error(err, kErrWaitTimeout); };
@@ -369,33 +455,42 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
         // ------------------------------------------------------------ copies
         const uint32_t lead = elect_one();
         const uint32_t full0 = smem_addr(&full[0]), a0 = smem_addr(sm + L::kOffA), b0 = smem_addr(sm + L::kOffB);
-        int s = 0, issued = 0;
-        uint32_t ph = 0;
+        Ring<ST> ring(1u);
+        int issued = 0;
         for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
             const Tile q = find_tile<NT>(tab, a, t, lane);
             const int nbox = GATHER ? 0 : (q.rows + 31) >> 5;
-            const uint32_t bytes = (a.fp4 ? L::kABytes / 2 : L::kABytes) + nbox * 4096;
+            const uint32_t bytes = (a.fp4 ? L::kASlice / 2 : L::kASlice) + nbox * 4096;  // per slice
             const int row = q.mt * kRowsPerTile;
             for (int kb = 0; kb < n_kb; kb++) {
-                ok = __all_sync(kFull, mbar_wait(&empty[s], ph ^ 1u, kWaitLimit));
+                ok = ring.wait(empty);
                 if (!ok) break;
+                ring.peek(empty);
+                const int s = ring.s;
                 const uint32_t bar = full0 + 8 * s, A = a0 + s * L::kABytes, B = b0 + s * L::kBBytes;
-                expect_bytes(lead, bar, bytes);
-                tma_load_3d(lead, A, &maps.w0, kb * kStageK, row, q.e, bar);
-                if (SWIGLU) tma_load_3d(lead, A + L::kABytes / 2, &maps.w1, kb * kStageK, row, q.e, bar);
-                if (!GATHER)
-                    for (int i = 0; i < nbox; i++)
-                        tma_load_2d(lead, B + i * 4096, &maps.x, kb * kStageK, q.r0 + 32 * i, bar);
-                issued++;
-                if (++s == ST) {
-                    s = 0;
-                    ph ^= 1u;
+                const int n = min(L::kSub, n_slices - L::kSub * kb);
+                expect_bytes(lead, bar, n * bytes);
+#pragma unroll
+                for (int sub = 0; sub < L::kSub; sub++) {
+                    if (sub >= n) break;
+                    const int k = (L::kSub * kb + sub) * kSliceK;
+                    const uint32_t As = A + sub * L::kASlice, Bs = B + sub * L::kBSlice;
+                    tma_load_3d(lead, As, &maps.w0, k, row, q.e, bar);
+                    if (SWIGLU) tma_load_3d(lead, As + L::kASlice / 2, &maps.w1, k, row, q.e, bar);
+                    if (!GATHER)
+                        for (int i = 0; i < nbox; i++) tma_load_2d(lead, Bs + i * 4096, &maps.x, k, q.r0 + 32 * i, bar);
                 }
+                issued++;
+                ring.next();
             }
         }
         if (!ok) {
             give_up();
-            // Let the copies in flight land before shared memory goes away.
+            // Let the copies in flight land before shared memory goes away:
+            // backwards over the stages issued last. (ring.ph is the parity of
+            // `empty`, the opposite of the one `full` completes with.)
+            int s = ring.s;
+            uint32_t ph = ring.ph ^ 1u;
             for (int i = 0; i < ST && i < issued; i++) {
                 if (s == 0) ph ^= 1u;
                 s = s == 0 ? ST - 1 : s - 1;
@@ -406,8 +501,8 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
         // ------------------------------------------------------ tensor cores
         const uint32_t lead = elect_one();
         const uint32_t empty0 = smem_addr(&empty[0]);
-        int s = 0, it = 0;
-        uint32_t ph = 0;
+        Ring<ST> ring(0u);
+        int it = 0;
         // A's type (5 = e2m1, 0 = e4m3), power-of-two scales, M.
         const uint32_t idesc0 = ((a.fp4 ? 5u : 0u) << 7) | (1u << 23) | ((kTileM >> 4) << 24);
         constexpr uint32_t kNextScale = (1u << 4) | (1u << 29);  // scale byte i of the word, B and A
@@ -424,26 +519,35 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
             const uint32_t idesc = idesc0 | ((uint32_t)((q.rows + 15) >> 4) << 18);  // N / 8 at bit 17
             const uint32_t d = tmem + b * NT;
             for (int kb = 0; kb < n_kb; kb++) {
-                ok = __all_sync(kFull, mbar_wait(&full[s], ph, kWaitLimit));
+                ok = ring.wait(full);
                 if (!ok) break;
+                ring.peek(full);
+                const int s = ring.s;
                 tc_fence_after();
                 fence_async_shared();
-                const uint32_t sfa = tmem + 2 * NT + s * L::kSfCols, sfb = sfa + 4;
-                tc_copy_scales(lead, sfa, sa0 + s * (L::kSfA >> 4));
+                // Scales of the slices side by side: A's 4 columns, then B's.
+                const uint32_t sf = tmem + 2 * NT + s * L::kSfCols;
 #pragma unroll
-                for (int j = 0; j < L::kBWords / 4; j++)
-                    tc_copy_scales(lead, sfb + 4 * j, sb0 + s * (L::kSfB >> 4) + j * 32);
-                const uint64_t ad = ad0 + s * (L::kABytes >> 4), bd = bd0 + s * (L::kBBytes >> 4);
-                const int nk = nk32 - 4 * kb;  // 32-element steps left
+                for (int sub = 0; sub < L::kSub; sub++) {
+                    tc_copy_scales(lead, sf + sub * (4 + L::kBWords), sa0 + ((s * L::kSfA + sub * 512) >> 4));
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (i < nk)
-                        tc_mma_mx(lead, d, ad + 2 * i, bd + 2 * i, idesc + i * kNextScale, sfa, sfb, (uint32_t)(kb | i));
-                tc_commit(lead, empty0 + 8 * s);
-                if (++s == ST) {
-                    s = 0;
-                    ph ^= 1u;
+                    for (int j = 0; j < L::kBWords; j += 4)
+                        tc_copy_scales(lead, sf + sub * (4 + L::kBWords) + 4 + j,
+                                       sb0 + ((s * L::kSfB + sub * L::kBWords * 128 + j * 128) >> 4));
                 }
+                const uint64_t ad = ad0 + s * (L::kABytes >> 4), bd = bd0 + s * (L::kBBytes >> 4);
+                const int nk = nk32 - 4 * L::kSub * kb;  // 32-element steps left
+#pragma unroll
+                for (int i = 0; i < 4 * L::kSub; i++) {
+                    const int sub = i >> 2;
+                    const uint32_t sfa = sf + sub * (4 + L::kBWords);
+                    if (i < nk)
+                        tc_mma_mx(lead, d, ad + sub * (L::kASlice >> 4) + 2 * (i & 3),
+                                  bd + sub * (L::kBSlice >> 4) + 2 * (i & 3), idesc + (i & 3) * kNextScale, sfa, sfa + 4,
+                                  (uint32_t)(kb | i));
+                }
+                tc_commit(lead, empty0 + 8 * s);
+                ring.next();
             }
             if (!ok) break;
             tc_commit(lead, smem_addr(&acc_full[b]));
@@ -463,66 +567,90 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
                 row[j] = (SWIGLU && j >= 2 ? a.w1_s : a.w0_s) + ((size_t)q.e * a.n_w + r) * nk32;
             }
         };
+        // B's row ids are read a tile ahead and resolved when the tile comes.
+        int raw[NT / 32];
+        auto read_ids = [&](int t) {
+            if (!GATHER || t >= total) return;
+            const Tile q = find_tile<NT>(tab, a, t, lane);
+#pragma unroll
+            for (int j = 0; j < NT / 32; j++) raw[j] = a.x_rows[q.r0 + min(lane + 32 * j, q.rows - 1)];
+        };
         auto rows_of_b = [&](const uint8_t *(&row)[NT / 32], int t) {
             const Tile q = find_tile<NT>(tab, a, t, lane);
 #pragma unroll
             for (int j = 0; j < NT / 32; j++) {
                 int x = q.r0 + min(lane + 32 * j, q.rows - 1);
-                if (a.x_rows) {
-                    x = a.x_rows[x];
-                    x = x < 0 ? -1 : x / a.x_div;
-                    x = x < 0 || x >= a.n_x ? 0 : x;
-                }
+                if (GATHER) x = x_row(raw[j], a);
                 row[j] = a.x_s + (size_t)x * nk32;
             }
+            read_ids(t + gridDim.x);
         };
-        ok = warp == 2 ? stage_scales<4, L::kSfA, ST>(rows_of_a, sm + L::kOffSfA, full, empty, total, n_kb, nk32, a.w_words, lane)
-                       : stage_scales<NT / 32, L::kSfB, ST>(rows_of_b, sm + L::kOffSfB, full, empty, total, n_kb, nk32,
-                                                           a.x_words, lane);
+#define DS3_SCALES(J, BYTES, MODE, rows_of, at) \
+    stage_scales<J, BYTES, L::kSub, ST, MODE>(rows_of, sm + at, full, empty, total, n_kb, nk32, lane)
+        if (warp == 2) {
+            ok = a.w_mode == 2   ? DS3_SCALES(4, L::kSfA, 2, rows_of_a, L::kOffSfA)
+                 : a.w_mode == 1 ? DS3_SCALES(4, L::kSfA, 1, rows_of_a, L::kOffSfA)
+                                 : DS3_SCALES(4, L::kSfA, 0, rows_of_a, L::kOffSfA);
+        } else {
+            read_ids(blockIdx.x);
+            ok = a.x_mode == 2   ? DS3_SCALES(NT / 32, L::kSfB, 2, rows_of_b, L::kOffSfB)
+                 : a.x_mode == 1 ? DS3_SCALES(NT / 32, L::kSfB, 1, rows_of_b, L::kOffSfB)
+                                 : DS3_SCALES(NT / 32, L::kSfB, 0, rows_of_b, L::kOffSfB);
+        }
+#undef DS3_SCALES
         if (!ok) give_up();
     } else if (GATHER && warp >= 12) {
         // ------------------------------------------------------- row gathers
-        // Warp g fills stages g, g + 4, ... of the CTA's sequence. Eight lanes
-        // copy a token row's 128 bytes, four rows per instruction.
+        // Every gathering warp works on every stage, in order: warp g copies the
+        // four-row groups g, g + 4, ... (Whole stages dealt out to the warps
+        // would let one of them run two uses of a slot ahead of a ring of fewer
+        // stages than warps, where a barrier's parity no longer tells the uses
+        // apart.) Eight lanes copy a token row's 128 bytes of a slice.
+        constexpr int kMine = NT / 4, kIds = (kMine + 31) / 32;
         const int g = warp - 12, piece = lane & 7, r4 = lane >> 3;
-        int *id = reinterpret_cast<int *>(sm + L::kOffIds) + g * NT;
-        int nid[NT / 32];
+        int *id = reinterpret_cast<int *>(sm + L::kOffIds) + g * kMine;
+        int nid[kIds];
         auto rows_of = [&](int t) {
             const Tile q = find_tile<NT>(tab, a, t, lane);
 #pragma unroll
-            for (int j = 0; j < NT / 32; j++) {
-                const int r = min(lane + 32 * j, q.rows - 1);
-                // A row id outside x reads row 0; the epilogue zeroes it.
-                int x = a.x_rows[q.r0 + r];
-                x = x < 0 ? -1 : x / a.x_div;
-                nid[j] = x < 0 || x >= a.n_x ? 0 : x;
+            for (int j = 0; j < kIds; j++) {
+                const int m = lane + 32 * j;  // the warp's m-th row
+                const int r = min((m >> 2) * 16 + 4 * g + (m & 3), q.rows - 1);
+                nid[j] = a.x_rows[q.r0 + r];
             }
             return q.rows;
         };
-        int t = blockIdx.x, seq = 0, rows = 0;  // seq: stages of this CTA before the tile
+        Ring<ST> ring(1u);
+        int t = blockIdx.x, rows = 0;
         if (t < total) rows = rows_of(t);
         for (; t < total && ok; t += gridDim.x) {
             __syncwarp();
 #pragma unroll
-            for (int j = 0; j < NT / 32; j++) id[lane + 32 * j] = nid[j];
+            for (int j = 0; j < kIds; j++)
+                if (lane + 32 * j < kMine) id[lane + 32 * j] = x_row(nid[j], a);
             __syncwarp();
             const int n = rows;
             if (t + (int)gridDim.x < total) rows = rows_of(t + gridDim.x);
-            for (int kb = (g - seq) & 3; kb < n_kb; kb += 4) {
-                const int s = (seq + kb) % ST;
-                ok = __all_sync(kFull, mbar_wait(&empty[s], ((uint32_t)(seq + kb) / ST & 1u) ^ 1u, kWaitLimit));
+            for (int kb = 0; kb < n_kb; kb++) {
+                ok = ring.wait(empty);
                 if (!ok) break;
-                const uint32_t dst = smem_addr(sm + L::kOffB + s * L::kBBytes) + r4 * 128;
-                const uint8_t *src = a.x + kb * kStageK + piece * 16;
-                if (kb * kStageK + piece * 16 < a.K) {
-#pragma unroll 4
-                    for (int i = 0; i < n; i += 4)  // the 128-byte swizzle: piece ^ (row % 8)
-                        cp_async16(dst + i * 128 + ((piece ^ ((i + r4) & 7)) << 4),
-                                   src + (size_t)(uint32_t)id[i + r4] * (uint32_t)a.K);
+                ring.peek(empty);
+                const int s = ring.s;
+#pragma unroll
+                for (int sub = 0; sub < L::kSub; sub++) {
+                    const int k = (L::kSub * kb + sub) * kSliceK + piece * 16;
+                    if (k >= a.K) break;
+                    const uint32_t dst = smem_addr(sm + L::kOffB + s * L::kBBytes + sub * L::kBSlice);
+                    const uint8_t *src = a.x + k;
+#pragma unroll 2
+                    for (int i = 4 * g, m = r4; i < n; i += 16, m += 4) {
+                        const int r = i + r4;  // the 128-byte swizzle: piece ^ (row % 8)
+                        cp_async16(dst + r * 128 + ((piece ^ (r & 7)) << 4), src + (size_t)(uint32_t)id[m] * (uint32_t)a.K);
+                    }
                 }
                 cp_async_arrive(&full[s]);
+                ring.next();
             }
-            seq += n_kb;
         }
         if (!ok) give_up();
         asm volatile("cp.async.wait_all;" ::: "memory");
@@ -674,7 +802,7 @@ bool encode(CUtensorMap *m, const void *base, int rank, uint64_t cols, uint64_t 
     const uint64_t row_bytes = fp4 ? cols / 2 : cols;
     const cuuint64_t dim[3] = {cols, rows, n};
     const cuuint64_t stride[2] = {row_bytes, row_bytes * rows};
-    const cuuint32_t box[3] = {kStageK, box_rows, 1};
+    const cuuint32_t box[3] = {kSliceK, box_rows, 1};
     const cuuint32_t step[3] = {1, 1, 1};
     EncodeTiled fn = encode_fn();
     return fn && fn(m, fp4 ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_UINT8, (cuuint32_t)rank,
@@ -683,12 +811,21 @@ bool encode(CUtensorMap *m, const void *base, int rank, uint64_t cols, uint64_t 
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-bool scale_words(const void *base, int n) { return ((uintptr_t)base | (uintptr_t)n) % 4 == 0; }
+// stage_scales' MODE for rows of n scales at `base`, `stage` scales per stage.
+int scale_mode(const void *base, int n, int stage)
+{
+    const uintptr_t v = (uintptr_t)base | (uintptr_t)n;
+    return v % stage == 0 ? 2 : v % 4 == 0 ? 1 : 0;
+}
 
 template <int NT, bool SWIGLU, bool GATHER>
-cudaError_t launch_nt(const LaunchCtx &c, const MoeMaps &maps, const MoeArgs &a)
+cudaError_t launch_nt(const LaunchCtx &c, const MoeMaps &maps, MoeArgs a)
 {
     using L = MoeLayout<NT>;
+    const int nk32 = a.K / kMxBlock, stage = 4 * L::kSub;  // scales of a row per stage
+    a.x_mode = scale_mode(a.x_s, nk32, stage);
+    a.w_mode = scale_mode(a.w0_s, nk32, stage);
+    if (SWIGLU) a.w_mode = min(a.w_mode, scale_mode(a.w1_s, nk32, stage));
     auto *k = moe_mx_k<NT, SWIGLU, GATHER>;
     static const cudaError_t set = [&] {
         keep_driver_carveout((const void *)k);
@@ -714,7 +851,6 @@ cudaError_t launch_moe_mx(const LaunchCtx &c, const MoeMxCall &q)
         !encode(&maps.w1, swiglu ? q.w1 : q.w0, 3, q.K, q.n_w, q.n_group, kTileM / 2, fp4) ||
         !encode(&maps.x, q.x, 2, q.K, q.n_x, 1, 32, false))
         return cudaErrorInvalidValue;
-    const int nk32 = q.K / kMxBlock;
     MoeArgs a = {};
     a.x = q.x;
     a.x_s = q.x_s;
@@ -735,8 +871,6 @@ cudaError_t launch_moe_mx(const LaunchCtx &c, const MoeMxCall &q)
     a.x_div = q.x_div;
     a.K = q.K;
     a.n_w = q.n_w;
-    a.x_words = scale_words(q.x_s, nk32);
-    a.w_words = scale_words(q.w0_s, nk32) && (!swiglu || scale_words(q.w1_s, nk32));
     const int rows_per_tile = swiglu ? kTileM / 2 : kTileM;
     a.n_mt = (unsigned)((q.n_w + rows_per_tile - 1) / rows_per_tile);
     a.n_mt_inv = (unsigned)(((1ull << 32) + a.n_mt - 1) / a.n_mt);

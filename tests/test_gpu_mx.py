@@ -336,6 +336,23 @@ def test_matmul_exact(ds3, B, rows, E, K, N, fmt, mapped):
     assert_bitexact(got, want, "out")
 
 
+@pytest.mark.parametrize("rows,E,K,N", [(3000, 60, 640, 1700), (3000, 14, 768, 2000), (6000, 12, 1024, 1500),
+                                        (9000, 40, 256, 1000)])
+@pytest.mark.parametrize("mapped", [False, True])
+def test_matmul_many_tiles_per_cta(ds3, B, rows, E, K, N, mapped):
+    """Several tiles for every CTA, at each token width the launcher picks, so
+    that the rings of stages wrap many times and across tiles."""
+    x, xs = exact_rows(1, rows, K, FP8)
+    w, ws = exact_rows(2, E * N, K, FP8)
+    w, ws = w.reshape(E, N, -1), ws.reshape(E, N, -1)
+    off = ragged(3, rows, E, 0.1)
+    src = I.rng(4).permutation(rows).astype(np.int32) if mapped else None
+    rc, got = run_matmul(ds3, B, x, xs, w, ws, FP8, off, rows, np.zeros((rows, N), np.float32), src)
+    assert rc == 0, ds3.last_error()
+    want = R.grouped(R.decode(x, xs, FP8), R.decode(w, ws, FP8), off, src if mapped else np.arange(rows))
+    assert_bitexact(got, want.astype(np.float32), "out")
+
+
 def test_matmul_rows_behind_the_last_group_are_left(ds3, B):
     x, xs = exact_rows(1, 40, 128, FP8)
     w, ws = exact_rows(2, 2 * 64, 128, FP8)
