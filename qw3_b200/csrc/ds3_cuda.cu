@@ -55,7 +55,8 @@ struct State {
     bool profile = false;
     bool pdl = true;  // DS3_CUDA_PDL=0 disables programmatic dependent launch
     // Library-owned device workspace: the fp32 copy of a router matrix stored
-    // in another type (moe_ffn_router*). Earlier, smaller allocations stay
+    // in another type (moe_ffn_router*), sorted token rows (moe_mx_*). Every use
+    // is written and read by consecutive launches on the one stream. Earlier, smaller allocations stay
     // alive until shutdown: graphs captured before a growth still use them.
     float *ws = nullptr;
     size_t ws_bytes = 0;
@@ -190,9 +191,10 @@ int finish(const char *op, cudaError_t launch, ProfScope &ps)
     return sync_and_check(op);
 }
 
-// At least `bytes` of library workspace, or nullptr (error set). It only
-// grows outside a graph capture (an allocation cannot be captured).
-float *workspace(const char *op, size_t bytes)
+// At least `bytes` of library workspace, or nullptr (error set, unless the
+// caller does not `need` it). It only grows outside a graph capture (an
+// allocation cannot be captured).
+float *workspace(const char *op, size_t bytes, bool need = true)
 {
     if (G.ws_bytes >= bytes) return G.ws;
     if (G.capturing) {
@@ -203,7 +205,8 @@ float *workspace(const char *op, size_t bytes)
     void *p = nullptr;
     const cudaError_t e = cudaMalloc(&p, bytes);
     if (e != cudaSuccess) {
-        set_error("%s: workspace of %zu bytes: %s", op, bytes, cudaGetErrorString(e));
+        if (need) set_error("%s: workspace of %zu bytes: %s", op, bytes, cudaGetErrorString(e));
+        else cudaGetLastError();
         return nullptr;
     }
     if (G.ws) G.ws_old.push_back(G.ws);
@@ -1526,6 +1529,10 @@ static int moe_mx_common(const char *op, const ds3_cuda_buffer_t *x_q, const ds3
     c.K = (int)n_in;
     c.n_w = (int)n_out;
     c.out_f16 = !swiglu && (int)out_type == 1;
+    // Scratch for sorted rows, when there is or can be enough: inside a capture
+    // it does not grow, and a failed allocation only means the slower gather.
+    const size_t scratch = ds3::moe_sort_bytes(c);
+    if (scratch && (G.ws_bytes >= scratch || !G.capturing)) c.sorted = (uint8_t *)workspace(op, scratch, false);
     ProfScope ps(op);
     return finish(op, ds3::launch_moe_mx(ctx(), c), ps);
 }

@@ -120,7 +120,9 @@ struct MoeMxCall {
     uint8_t *out_s;
     int w_type, n_x, x_div, n_rows, n_out_rows, n_group, K, n_w;
     bool out_f16;
+    uint8_t *sorted;  // moe_sort_bytes(q) of scratch, or nullptr: gather inside the kernel
 };
+size_t moe_sort_bytes(const MoeMxCall &q);
 cudaError_t launch_moe_mx(const LaunchCtx &c, const MoeMxCall &q);
 
 cudaError_t launch_bounded_wait_selftest(const LaunchCtx &c, uint32_t polls);

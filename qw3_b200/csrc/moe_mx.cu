@@ -368,8 +368,8 @@ __device__ __forceinline__ bool stage_scales(Rows &rows_of, uint8_t *dst, uint64
 }
 
 // SWIGLU: w0 / w1 are the gate / up weights and out is MXFP8. Otherwise w0
-// alone, and out is fp32 or fp16. GATHER: token rows come through x_rows;
-// otherwise sorted row r is row r of x.
+// alone, and out is fp32 or fp16. GATHER: the kernel fetches token rows through
+// x_rows; otherwise sorted row r is row r of x.
 template <int NT, bool SWIGLU, bool GATHER>
 __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_constant__ MoeMaps maps, const MoeArgs a,
                                                            unsigned *err)
@@ -673,7 +673,7 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
                 const int r = q.r0 + me;
                 int xid = r;
                 bool good = true;
-                if (GATHER) {
+                if (a.x_rows) {
                     xid = a.x_rows[r];
                     good = xid >= 0 && xid / a.x_div < a.n_x;
                     if (!good) flag_error(err, kErrBadId);
@@ -776,6 +776,29 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::kTmemCols) : "memory");
 }
 
+// x rows and their scales in sorted order: one warp per row, 16 bytes a lane.
+__global__ void __launch_bounds__(256) moe_sort_rows_k(const uint8_t *sorted_x, const uint8_t *sorted_s, const MoeArgs a)
+{
+    pdl_wait();
+    pdl_trigger();
+    const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (r >= min(a.offsets[a.n_group], a.n_rows)) return;  // rows behind the last group are not read
+    const size_t x = x_row(a.x_rows[r], a);
+    const uint4 *src = reinterpret_cast<const uint4 *>(a.x + x * a.K);
+    uint4 *dst = reinterpret_cast<uint4 *>(const_cast<uint8_t *>(sorted_x) + (size_t)r * a.K);
+#pragma unroll 4
+    for (int i = lane; i < a.K / 16; i += 32) dst[i] = src[i];
+    const int nk32 = a.K / kMxBlock;
+    const uint8_t *s = a.x_s + x * nk32;
+    uint8_t *d = const_cast<uint8_t *>(sorted_s) + (size_t)r * nk32;
+    if (a.x_mode) {
+        for (int i = lane; i < nk32 / 4; i += 32)
+            reinterpret_cast<uint32_t *>(d)[i] = reinterpret_cast<const uint32_t *>(s)[i];
+    } else {
+        for (int i = lane; i < nk32; i += 32) d[i] = s[i];
+    }
+}
+
 // ---------------------------------------------------------------- host side
 typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
@@ -841,16 +864,24 @@ cudaError_t launch_nt(const LaunchCtx &c, const MoeMaps &maps, MoeArgs a)
 
 }  // namespace
 
+static int moe_mean_rows(int n_rows, int n_group) { return (n_rows + n_group - 1) / n_group; }
+
+// Gathering inside the product kernel goes through the threads' copy path,
+// which cannot feed wide tiles; sorting the rows first costs a pass over them.
+// Measured, 128 groups, 2048 -> 2 x 768, gathered / in place, us: mean 32 rows
+// 52 / 50, 64: 70 / 61, 128: 116 / 83, 256: 200 / 151; the sort is 5 us at 64.
+size_t moe_sort_bytes(const MoeMxCall &q)
+{
+    if (!q.x_rows || moe_mean_rows(q.n_rows, q.n_group) <= 48) return 0;
+    return (size_t)q.n_rows * q.K + (size_t)q.n_rows * (q.K / kMxBlock);
+}
+
 cudaError_t launch_moe_mx(const LaunchCtx &c, const MoeMxCall &q)
 {
     if (q.n_rows <= 0 || q.n_group <= 0) return cudaSuccess;
     if (q.n_group > kMaxGroups) return cudaErrorInvalidValue;
     MoeMaps maps;
     const bool fp4 = q.w_type == kMxFp4, swiglu = q.w1 != nullptr;
-    if (!encode(&maps.w0, q.w0, 3, q.K, q.n_w, q.n_group, swiglu ? kTileM / 2 : kTileM, fp4) ||
-        !encode(&maps.w1, swiglu ? q.w1 : q.w0, 3, q.K, q.n_w, q.n_group, kTileM / 2, fp4) ||
-        !encode(&maps.x, q.x, 2, q.K, q.n_x, 1, 32, false))
-        return cudaErrorInvalidValue;
     MoeArgs a = {};
     a.x = q.x;
     a.x_s = q.x_s;
@@ -874,11 +905,30 @@ cudaError_t launch_moe_mx(const LaunchCtx &c, const MoeMxCall &q)
     const int rows_per_tile = swiglu ? kTileM / 2 : kTileM;
     a.n_mt = (unsigned)((q.n_w + rows_per_tile - 1) / rows_per_tile);
     a.n_mt_inv = (unsigned)(((1ull << 32) + a.n_mt - 1) / a.n_mt);
-    const int avg = (q.n_rows + q.n_group - 1) / q.n_group;
-    const int nt = avg <= 64 ? 64 : avg <= 256 ? 128 : 224;
-#define DS3_MOE(NT)                                                                                       \
-    (swiglu ? (q.x_rows ? launch_nt<NT, true, true>(c, maps, a) : launch_nt<NT, true, false>(c, maps, a)) \
-            : (q.x_rows ? launch_nt<NT, false, true>(c, maps, a) : launch_nt<NT, false, false>(c, maps, a)))
+    int n_map = q.n_x;
+    const bool sorted = q.x_rows && q.sorted;
+    if (sorted) {
+        uint8_t *sx = q.sorted, *ss = q.sorted + (size_t)q.n_rows * q.K;
+        a.x_mode = scale_mode(q.x_s, q.K / kMxBlock, 4);
+        launch_k(c, moe_sort_rows_k, dim3((unsigned)((q.n_rows + 7) / 8)), dim3(256), sx, ss, a);
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+        a.x = sx;
+        a.x_s = ss;
+        n_map = q.n_rows;
+    }
+    if (!encode(&maps.w0, q.w0, 3, q.K, q.n_w, q.n_group, swiglu ? kTileM / 2 : kTileM, fp4) ||
+        !encode(&maps.w1, swiglu ? q.w1 : q.w0, 3, q.K, q.n_w, q.n_group, kTileM / 2, fp4) ||
+        !encode(&maps.x, a.x, 2, q.K, n_map, 1, 32, false))
+        return cudaErrorInvalidValue;
+    // Token columns per tile by the groups' mean size. Measured over 128 groups,
+    // 2048 -> 2 x 768, us at 64 / 128 / 224 columns: mean 64: 70 / 61 / 71, 96:
+    // 91 / 68 / 75, 128: 113 / 95 / 83, 256: 205 / 158 / 151.
+    const int avg = moe_mean_rows(q.n_rows, q.n_group);
+    const int nt = avg <= 48 ? 64 : avg <= 112 ? 128 : 224;
+#define DS3_MOE(NT)                                                                                                  \
+    (swiglu ? (q.x_rows && !sorted ? launch_nt<NT, true, true>(c, maps, a) : launch_nt<NT, true, false>(c, maps, a)) \
+            : (q.x_rows && !sorted ? launch_nt<NT, false, true>(c, maps, a) : launch_nt<NT, false, false>(c, maps, a)))
     return nt == 64 ? DS3_MOE(64) : nt == 128 ? DS3_MOE(128) : DS3_MOE(224);
 #undef DS3_MOE
 }
