@@ -78,7 +78,8 @@ struct MoeLayout {
     static constexpr int kOffXch = kOffSfB + kStages * kSfB;
     static constexpr int kOffTab = kOffXch + kXch;        // first row, rows, first tile and block size of each group
     static constexpr int kOffIds = kOffTab + 4 * kMaxGroups * 4;  // gathered row ids, per gathering warp
-    static constexpr int kOffCol = kOffIds + NT * 4;                    // epilogue columns, two tiles
+    static constexpr int kOffCol = kOffIds + NT * 4;              // epilogue columns, two tiles (16-byte reads)
+    static_assert(kOffCol % 16 == 0 && NT % 16 == 0, "layout");
     static constexpr int kUsed = kOffCol + 2 * NT * 8;
     static constexpr size_t kSmem = kUsed + 1024;         // the base is aligned up to 1024
     static constexpr int kSfCols = kSub * (4 + kBWords);
@@ -104,7 +105,7 @@ struct MoeArgs {
     int n_x, n_rows, n_out_rows, n_group, x_div, K, n_w;
     int x_mode, w_mode;        // how scale rows are loaded (stage_scales)
     unsigned n_mt, n_mt_inv;   // weight blocks per group, 2^32 / n_mt rounded up
-    int half, fp4;             // out is fp16; the weights are MXFP4
+    int half, fp4;             // out is fp16 (2: pairs are aligned); the weights are MXFP4
 };
 
 // ------------------------------------------------------------ PTX wrappers
@@ -219,8 +220,9 @@ __device__ __forceinline__ void tc_ld16(uint32_t (&v)[16], uint32_t tmem)
         : "r"(tmem)
         : "memory");
 }
-// Shared-memory writes by threads (scales, gathered rows) that this thread has
-// seen through a barrier are seen by the tensor-core work it issues after this.
+// Between shared-memory writes by threads and the tensor core's reads of them:
+// by the writer before it arrives (scales; its warp has the time), or, for rows
+// whose copies land after their thread has gone on, by the issuing warp.
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // Whether `ok` holds in all `threads` threads that meet at barrier `id`.
 __device__ __forceinline__ bool named_all(int id, int threads, bool ok)
@@ -354,6 +356,7 @@ __device__ __forceinline__ bool stage_scales(Rows &rows_of, uint8_t *dst, uint64
                         *reinterpret_cast<uint4 *>(dst + ring.s * BYTES + i * (BYTES / SUB) + j * 128 + lane * 16) =
                             make_uint4(w(0), w(1), w(2), w(3));
                     }
+                fence_async_shared();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[ring.s]);
                 ring.next();
@@ -524,7 +527,7 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
                 ring.peek(full);
                 const int s = ring.s;
                 tc_fence_after();
-                fence_async_shared();
+                if (GATHER) fence_async_shared();  // the rows the gathering warps copied
                 // Scales of the slices side by side: A's 4 columns, then B's.
                 const uint32_t sf = tmem + 2 * NT + s * L::kSfCols;
 #pragma unroll
@@ -669,6 +672,7 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
             // goes (-1: nowhere; SwiGLU: its weight) and whether its token row
             // is one of x. Two buffers: no thread is two tiles ahead of another.
             int2 *col = reinterpret_cast<int2 *>(sm + L::kOffCol) + b * NT;
+            if (me >= q.rows && me < NT) col[me] = make_int2(-1, 0);
             if (me < q.rows) {
                 const int r = q.r0 + me;
                 int xid = r;
@@ -718,48 +722,69 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
                     for (int i = 0; i < 8; i++) mine[i * 32 + lane] = __uint_as_float(gate ? v[2 * i + 1] : v[2 * i]);
                     named_sync(4 + side * 2 + (w & 1), 64);
                     const int f0 = q.mt * kRowsPerTile + 32 * (w & 1);
-                    uint32_t my_scale = 0;
+                    // No branches over the columns, so that the eight run side by
+                    // side: a column alone is 300 cycles of latencies.
+                    float h[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float other = theirs[i * 32 + lane];
+                        const float gv = gate ? __uint_as_float(v[2 * i]) : other;
+                        const float uv = gate ? other : __uint_as_float(v[2 * i + 1]);
+                        const int2 k = col[c0 + 2 * i + (gate ? 0 : 1)];
+                        // silu(g) u: the quotient is good to 2 ulp, far inside the 8-bit rounding.
+                        h[i] = __fdividef(gv, 1.0f + expf(-gv)) * uv;
+                        if (a.row_w) h[i] *= __int_as_float(k.x);
+                        if (!k.y) h[i] = 0.0f;
+                    }
+                    uint32_t sc[8], my_scale = 0;
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        sc[i] = mx_scale<kMxEmaxFp8>(__reduce_max_sync(kFull, __float_as_uint(h[i]) & 0x7fffffffu));
                     uint8_t *oq = reinterpret_cast<uint8_t *>(a.out) + (size_t)(q.r0 + c0) * a.n_w + f0 + lane;
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         const int c = 2 * i + (gate ? 0 : 1);
-                        if (c >= nc) break;
-                        const float other = theirs[i * 32 + lane];
-                        const float gv = gate ? __uint_as_float(v[2 * i]) : other;
-                        const float uv = gate ? other : __uint_as_float(v[2 * i + 1]);
-                        const int2 k = col[c0 + c];
-                        // silu(g) u: the quotient is good to 2 ulp, far inside the 8-bit rounding.
-                        float h = __fdividef(gv, 1.0f + expf(-gv)) * uv;
-                        if (a.row_w) h *= __int_as_float(k.x);
-                        if (!k.y) h = 0.0f;
-                        const uint32_t amax = __reduce_max_sync(kFull, __float_as_uint(h) & 0x7fffffffu);
-                        const uint32_t sc = mx_scale<kMxEmaxFp8>(amax);
-                        const uint32_t e = e4m3x2(mx_scaled(h, sc, mx_inv_scale(sc)), 0.0f);
-                        if (lane == c) my_scale = sc;
-                        if (f0 < a.n_w) oq[(size_t)c * a.n_w] = (uint8_t)e;
+                        const uint32_t e = e4m3x2(mx_scaled(h[i], sc[i], mx_inv_scale(sc[i])), 0.0f);
+                        if (lane == c) my_scale = sc[i];
+                        if (c < nc && f0 < a.n_w) oq[(size_t)c * a.n_w] = (uint8_t)e;
                     }
                     if ((lane & 1) == (gate ? 0 : 1) && lane < nc && f0 < a.n_w)
                         a.out_s[(size_t)(q.r0 + c0 + lane) * (a.n_w / kMxBlock) + f0 / kMxBlock] = (uint8_t)my_scale;
                 } else {
                     const int m = q.mt * kRowsPerTile + 32 * w + lane;
                     const bool in = m < a.n_w;
-                    if (a.half) {
-                        __half *o = reinterpret_cast<__half *>(a.out) + m;
+                    // All columns' places first, two to a load; then stores that
+                    // wait for nothing (one by one, a column took 80 cycles).
+                    int4 k[8];
 #pragma unroll
-                        for (int c = 0; c < 16; c++) {
-                            if (c >= nc) break;
-                            const int2 k = col[c0 + c];
-                            if (k.x >= 0 && in)
-                                o[(size_t)(uint32_t)k.x * (uint32_t)a.n_w] = __float2half_rn(k.y ? __uint_as_float(v[c]) : 0.0f);
+                    for (int i = 0; i < 8; i++) k[i] = reinterpret_cast<const int4 *>(col + c0)[i];
+                    if (a.half) {
+                        // Two columns at a time: an even lane stores its row and the
+                        // next of the first column, an odd lane of the second.
+                        __half *o = reinterpret_cast<__half *>(a.out);
+                        const int odd = lane & 1;
+#pragma unroll
+                        for (int c = 0; c < 16; c += 2) {
+                            const float v0 = k[c / 2].y ? __uint_as_float(v[c]) : 0.0f;
+                            const float v1 = k[c / 2].w ? __uint_as_float(v[c + 1]) : 0.0f;
+                            const float got = __shfl_xor_sync(kFull, odd ? v0 : v1, 1);
+                            const int to = odd ? k[c / 2].z : k[c / 2].x;
+                            const __half2 pair = odd ? __floats2half2_rn(got, v1) : __floats2half2_rn(v0, got);
+                            __half *at = o + (size_t)(uint32_t)to * (uint32_t)a.n_w + (m - odd);
+                            if (to >= 0 && a.half == 2 && m - odd < a.n_w) {
+                                *reinterpret_cast<__half2 *>(at) = pair;
+                            } else if (to >= 0) {  // rows of an odd length, or an odd base
+                                if (m - odd < a.n_w) at[0] = __low2half(pair);
+                                if (m - odd + 1 < a.n_w) at[1] = __high2half(pair);
+                            }
                         }
                     } else {
                         float *o = reinterpret_cast<float *>(a.out) + m;
 #pragma unroll
                         for (int c = 0; c < 16; c++) {
-                            if (c >= nc) break;
-                            const int2 k = col[c0 + c];
-                            if (k.x >= 0 && in)
-                                o[(size_t)(uint32_t)k.x * (uint32_t)a.n_w] = k.y ? __uint_as_float(v[c]) : 0.0f;
+                            const int to = c & 1 ? k[c / 2].z : k[c / 2].x, good = c & 1 ? k[c / 2].w : k[c / 2].y;
+                            if (to >= 0 && in)
+                                o[(size_t)(uint32_t)to * (uint32_t)a.n_w] = good ? __uint_as_float(v[c]) : 0.0f;
                         }
                     }
                 }
@@ -885,7 +910,8 @@ cudaError_t launch_moe_mx(const LaunchCtx &c, const MoeMxCall &q)
     MoeArgs a = {};
     a.x = q.x;
     a.x_s = q.x_s;
-    a.half = q.out_f16;
+    // Pairs of an fp16 row are whole words when the row length is even and the base aligned.
+    a.half = !q.out_f16 ? 0 : q.n_w % 2 == 0 && (uintptr_t)q.out % 4 == 0 ? 2 : 1;
     a.fp4 = fp4;
     a.w0_s = q.w0_s;
     a.w1_s = q.w1_s;

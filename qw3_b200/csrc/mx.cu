@@ -109,12 +109,138 @@ __global__ void __launch_bounds__(256) mx_dequantize_k(const uint8_t *q, const u
 // which jump where a value crosses a rounding border, then do not depend on
 // the order of the sum.
 //
-// One warp per row; x and r rows are staged in shared memory by bulk copies
-// (TMA, 1-D) on an mbarrier, NS rows deep, as in add_rms_norm_bulk. The row
-// stays in shared memory for the two passes (squares, output). Lane l works on
-// elements 4 l .. 4 l + 3 of every 128: an MX block is 8 lanes.
+// Up to 4096 elements: four warps per row, the row in registers (VPT float4 of
+// x and of r per thread, all loads issued before the first use), so the reads
+// and writes of other rows pass under a row's reductions. Thread t works on
+// elements 4 t .. 4 t + 3 of every 512: an MX block is 8 neighbouring lanes.
+// One warp per row with the row in shared memory, the first version, kept too
+// few reads in flight behind its chains (16384 x 2048: 149 us).
+// Longer rows: that version, below.
 constexpr int kNormMxMaxN = 16384;
 
+// 1 / sqrt(m) to full fp64 accuracy: the fp32 estimate and two Newton steps,
+// each of which squares its relative error (2^-22 at first).
+__device__ __forceinline__ double inv_sqrt64(double m)
+{
+    if (!(m > 1e-30 && m < 1e30)) return 1.0 / sqrt(m);
+    double y = rsqrtf((float)m);
+    y = y * fma(-0.5 * m * y, y, 1.5);
+    return y * fma(-0.5 * m * y, y, 1.5);
+}
+
+// Four normed values s * inv * g, inv = ih + il, each rounded once.
+__device__ __forceinline__ float4 norm4(float4 s, double inv, float ih, float il, float4 g)
+{
+    const float a[4] = {__fmul_rn(s.x, ih), __fmul_rn(s.y, ih), __fmul_rn(s.z, ih), __fmul_rn(s.w, ih)};
+    const float low = fminf(fminf(fabsf(a[0]), fabsf(a[1])), fminf(fabsf(a[2]), fabsf(a[3])));
+    // Below 2^-100 the carried errors would leave fp32's range: products in fp64.
+    if (inv < 0x1p-100 || low < 0x1p-100f)
+        return make_float4((float)((double)s.x * inv * (double)g.x), (float)((double)s.y * inv * (double)g.y),
+                           (float)((double)s.z * inv * (double)g.z), (float)((double)s.w * inv * (double)g.w));
+    auto one = [&](float x, float a, float g) {
+        const float ae = fmaf(x, il, fmaf(x, ih, -a));
+        const float h = __fmul_rn(a, g);
+        return __fadd_rn(h, fmaf(ae, g, fmaf(a, g, -h)));
+    };
+    return make_float4(one(s.x, a[0], g.x), one(s.y, a[1], g.y), one(s.z, a[2], g.z), one(s.w, a[3], g.w));
+}
+
+__device__ __forceinline__ uint32_t amax4(float4 v)
+{
+    return max(max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu),
+               max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
+}
+
+__device__ __forceinline__ uint32_t quant4(float4 v, uint32_t sc)
+{
+    const float inv = mx_inv_scale(sc);
+    return e4m3x4(mx_scaled(v.x, sc, inv), mx_scaled(v.y, sc, inv), mx_scaled(v.z, sc, inv), mx_scaled(v.w, sc, inv));
+}
+
+__device__ __forceinline__ double sumsq4(float4 v, double acc)
+{
+    acc = fma((double)v.x, (double)v.x, acc);
+    acc = fma((double)v.y, (double)v.y, acc);
+    acc = fma((double)v.z, (double)v.z, acc);
+    return fma((double)v.w, (double)v.w, acc);
+}
+
+template <int VPT>
+__global__ void __launch_bounds__(128) add_rms_norm_mx_row(const float *x, const float *r, const float *w, float *sum_out,
+                                                           float *norm_out, uint8_t *q, uint8_t *scales, int n, float eps)
+{
+    __shared__ double part[4];
+    const int tid = threadIdx.x, n4 = n / 4;
+    const int64_t row = blockIdx.x;
+    if (tid < 2) {  // the row, into L2 while the previous kernel runs
+        const float *p = tid ? r : x;
+        if (p) prefetch_l2(p + row * n, (uint64_t)n * 4);
+    }
+    pdl_wait();
+    pdl_trigger();
+    const float4 *xr = reinterpret_cast<const float4 *>(x + row * n), *w4 = reinterpret_cast<const float4 *>(w);
+    float4 v[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; i++) {
+        v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (tid + 128 * i < n4) v[i] = ld_stream_inflight(xr + tid + 128 * i);
+    }
+    if (r) {
+        const float4 *rr = reinterpret_cast<const float4 *>(r + row * n);
+        float4 b[VPT];
+#pragma unroll
+        for (int i = 0; i < VPT; i++) {
+            b[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (tid + 128 * i < n4) b[i] = ld_stream_inflight(rr + tid + 128 * i);
+        }
+#pragma unroll
+        for (int i = 0; i < VPT; i++) v[i] = f4_add(v[i], b[i]);
+    }
+    if (sum_out) {
+        float4 *so = reinterpret_cast<float4 *>(sum_out + row * n);
+#pragma unroll
+        for (int i = 0; i < VPT; i++)
+            if (tid + 128 * i < n4) so[tid + 128 * i] = v[i];
+    }
+    double ss = 0.0;
+#pragma unroll
+    for (int i = 0; i < VPT; i++) ss += sumsq4(v[i], 0.0);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
+    if ((tid & 31) == 0) part[tid >> 5] = ss;
+    __syncthreads();
+    ss = (part[0] + part[1]) + (part[2] + part[3]);
+    const double inv = inv_sqrt64(ss / (double)n + (double)eps);
+    const float ih = (float)inv, il = (float)(inv - (double)ih);
+    float4 *no = norm_out ? reinterpret_cast<float4 *>(norm_out + row * n) : nullptr;
+    uint32_t *qo = reinterpret_cast<uint32_t *>(q + row * n);
+    uint8_t *sco = scales + row * (n / kMxBlock);
+    uint32_t amax[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; i++) {
+        const int c = tid + 128 * i;
+        if (c < n4) {
+            v[i] = norm4(v[i], inv, ih, il, ld_param(w4 + c));
+            if (no) no[c] = v[i];
+        }
+        amax[i] = amax4(v[i]);
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1)
+#pragma unroll
+        for (int i = 0; i < VPT; i++) amax[i] = max(amax[i], __shfl_xor_sync(kFull, amax[i], o));
+#pragma unroll
+    for (int i = 0; i < VPT; i++) {
+        const int c = tid + 128 * i;
+        if (c >= n4) break;
+        const uint32_t sc = mx_scale<kMxEmaxFp8>(amax[i]);
+        qo[c] = quant4(v[i], sc);
+        if ((tid & 7) == 0) sco[c >> 3] = (uint8_t)sc;
+    }
+}
+
+// Rows longer than 4096: one warp per row, staged in shared memory by bulk
+// copies (TMA, 1-D) on an mbarrier, NS rows deep, as in add_rms_norm_bulk.
 template <int NS>
 __global__ void __launch_bounds__(32) add_rms_norm_mx_k(const float *x, const float *r, const float *w, float *sum_out,
                                                         float *norm_out, uint8_t *q, uint8_t *scales, int n, int64_t rows,
@@ -170,46 +296,31 @@ __global__ void __launch_bounds__(32) add_rms_norm_mx_k(const float *x, const fl
                 xs[i] = v;  // read back by this lane below
             }
             if (so) so[i] = v;
-            ss = fma((double)v.x, (double)v.x, ss);
-            ss = fma((double)v.y, (double)v.y, ss);
-            ss = fma((double)v.z, (double)v.z, ss);
-            ss = fma((double)v.w, (double)v.w, ss);
+            ss += sumsq4(v, 0.0);
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
-        const double inv = 1.0 / sqrt(ss / (double)n + (double)eps);
+        const double inv = inv_sqrt64(ss / (double)n + (double)eps);
         const float ih = (float)inv, il = (float)(inv - (double)ih);
         const float4 *w4 = reinterpret_cast<const float4 *>(w);
         float4 *no = norm_out ? reinterpret_cast<float4 *>(norm_out + cur * n) : nullptr;
         uint32_t *qo = reinterpret_cast<uint32_t *>(q + cur * n);
         uint8_t *sco = scales + cur * (n / kMxBlock);
-        // Below 2^-100 the carried errors would leave fp32's range: products in fp64.
-        const bool tiny = inv < 0x1p-100;
-        auto norm1 = [&](float s, float g) {
-            const float a = __fmul_rn(s, ih);
-            if (tiny || fabsf(a) < 0x1p-100f) return (float)((double)s * inv * (double)g);
-            const float ae = fmaf(s, il, fmaf(s, ih, -a));
-            const float h = __fmul_rn(a, g);
-            return __fadd_rn(h, fmaf(ae, g, fmaf(a, g, -h)));
-        };
 #pragma unroll 2
         for (int i0 = 0; i0 < n / 4; i0 += 32) {  // whole warps: the shuffles need every lane
             const int i = i0 + lane;
             const bool in = i < n / 4;
             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (in) {
-                const float4 s = xs[i], g = ld_param(w4 + i);
-                v = make_float4(norm1(s.x, g.x), norm1(s.y, g.y), norm1(s.z, g.z), norm1(s.w, g.w));
+                v = norm4(xs[i], inv, ih, il, ld_param(w4 + i));
                 if (no) no[i] = v;
             }
-            uint32_t amax = max(max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu),
-                                max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
+            uint32_t amax = amax4(v);
 #pragma unroll
             for (int o = 1; o < 8; o <<= 1) amax = max(amax, __shfl_xor_sync(kFull, amax, o));
             if (!in) continue;
             const uint32_t sc = mx_scale<kMxEmaxFp8>(amax);
-            const float is = mx_inv_scale(sc);
-            qo[i] = e4m3x4(mx_scaled(v.x, sc, is), mx_scaled(v.y, sc, is), mx_scaled(v.z, sc, is), mx_scaled(v.w, sc, is));
+            qo[i] = quant4(v, sc);
             if ((lane & 7) == 0) sco[i >> 3] = (uint8_t)sc;
         }
         // Slot free for the next copy: this warp's reads and writes of it come first.
@@ -281,6 +392,15 @@ cudaError_t launch_add_rms_norm_mx(const LaunchCtx &c, const float *x, const flo
 {
     if (rows <= 0) return cudaSuccess;
     if (n <= 0 || n % kMxBlock || n > kNormMxMaxN) return cudaErrorInvalidValue;
+    if (n <= 4096) {
+        if (rows > 0x7fffffffLL) return cudaErrorInvalidValue;
+        const dim3 g((unsigned)rows), b(128);
+        if (n <= 512) launch_k(c, add_rms_norm_mx_row<1>, g, b, x, r, w, sum_out, norm_out, q, scales, n, eps);
+        else if (n <= 1024) launch_k(c, add_rms_norm_mx_row<2>, g, b, x, r, w, sum_out, norm_out, q, scales, n, eps);
+        else if (n <= 2048) launch_k(c, add_rms_norm_mx_row<4>, g, b, x, r, w, sum_out, norm_out, q, scales, n, eps);
+        else launch_k(c, add_rms_norm_mx_row<8>, g, b, x, r, w, sum_out, norm_out, q, scales, n, eps);
+        return cudaGetLastError();
+    }
     // Two rows in flight per warp when a warp has more than one and they fit.
     if (rows > c.n_sm && n <= kNormMxMaxN / 2)
         return run_norm_mx<2>(c, x, r, w, sum_out, norm_out, q, scales, n, rows, eps);
