@@ -106,66 +106,101 @@ __global__ void __launch_bounds__(kRouteThreads) moe_expert_lists_k(
 
 // Sorted rows without list capacities: entries (token * n_used + slot) in
 // expert order, each expert's in ascending order, and the experts' bounds.
-// One CTA per expert. Thread t owns a contiguous run of entries: it counts
-// those of smaller experts and of its own, one CTA-wide scan places its run,
-// and a second walk over the run (from L2) writes the hits out. offsets[ex] is
-// the number of entries of smaller experts, so no CTA waits for another.
+// One CTA per expert, no CTA waits for another: offsets[ex] is the number of
+// entries of smaller experts, which each CTA counts itself. A chunk of entries
+// is read once, coalesced (4 per thread and load, all loads of a chunk
+// independent), and leaves one bit per entry in shared memory (is it this
+// expert's); a thread then owns 64 consecutive bits, one CTA-wide scan of the
+// bit counts places its hits, and it writes them out in order. 65,528 entries,
+// 128 experts: 26 us when each thread walked its own run of entries twice.
+constexpr int kRowsChunk = 64 * kRouteThreads;  // entries per pass
+
 __global__ void __launch_bounds__(kRouteThreads) moe_expert_rows_k(const int32_t *idx, int32_t *offsets, int32_t *entries,
-                                                                   int32_t *row_of, int n_entries, int n_expert, int run,
-                                                                   int vec, unsigned *err)
+                                                                   int32_t *row_of, int n_entries, int n_expert, int vec,
+                                                                   unsigned *err)
 {
+    __shared__ uint32_t bits[kRowsChunk / 32];
     __shared__ int32_t wpre[kRouteWarps], wless[kRouteWarps];
     pdl_wait();
     pdl_trigger();
     const int ex = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int lo = min(n_entries, tid * run), hi = min(n_entries, lo + run);  // run % 4 == 0
-    auto walk = [&](auto &&f) {
-        int i = lo;
-        if (vec) {
-#pragma unroll 4
-            for (; i + 4 <= hi; i += 4) {
-                const int4 e = *reinterpret_cast<const int4 *>(idx + i);
-                f(i, e.x);
-                f(i + 1, e.y);
-                f(i + 2, e.z);
-                f(i + 3, e.w);
-            }
+    auto read4 = [&](int i) {  // ids of entries i .. i + 3, -1 behind the last
+        int4 e = make_int4(-1, -1, -1, -1);
+        if (vec && i + 4 <= n_entries) {
+            e = *reinterpret_cast<const int4 *>(idx + i);
+        } else {
+            if (i < n_entries) e.x = idx[i];
+            if (i + 1 < n_entries) e.y = idx[i + 1];
+            if (i + 2 < n_entries) e.z = idx[i + 2];
+            if (i + 3 < n_entries) e.w = idx[i + 3];
         }
-        for (; i < hi; i++) f(i, idx[i]);
+        return e;
     };
-    int mine = 0, less = 0;
-    walk([&](int i, int e) {
-        mine += e == ex;
-        less += e >= 0 && e < ex;
-        if (ex == 0 && (e < 0 || e >= n_expert)) {
-            flag_error(err, kErrBadId);
-            if (row_of) row_of[i] = -1;
-        }
-    });
-    int inc = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(kFull, inc, o);
-        if (lane >= o) inc += y;
+    auto lower = [&](int e) { return (int)(e >= 0 && e < ex); };
+    int less = 0;
+    // Entries behind the first chunk count before anything can be placed.
+    for (int i = kRowsChunk + 4 * tid; i < n_entries; i += 4 * kRouteThreads) {
+        const int4 e = read4(i);
+        less += lower(e.x) + lower(e.y) + lower(e.z) + lower(e.w);
     }
-    less = __reduce_add_sync(kFull, less);
-    if (lane == 31) wpre[warp] = inc;
-    if (lane == 0) wless[warp] = less;
-    __syncthreads();
-    const int in_warp = wpre[lane];
-    const int first = __reduce_add_sync(kFull, wless[lane]);               // entries of smaller experts
-    const int before = __reduce_add_sync(kFull, lane < warp ? in_warp : 0);  // this expert's, in earlier warps
-    int row = first + before + inc - mine;
-    if (mine)
-        walk([&](int i, int e) {
-            if (e != ex) return;
+    int base = 0;  // this expert's entries in earlier chunks
+    for (int c0 = 0; c0 == 0 || c0 < n_entries; c0 += kRowsChunk) {
+        const int n = min(n_entries - c0, kRowsChunk);
+#pragma unroll 4
+        for (int j = 0; j < n; j += 4 * kRouteThreads) {
+            const int i = c0 + j + 4 * tid;
+            const int4 e = read4(i);
+            uint32_t hit = (e.x == ex) | (e.y == ex) << 1 | (e.z == ex) << 2 | (e.w == ex) << 3;
+            if (c0 == 0) less += lower(e.x) + lower(e.y) + lower(e.z) + lower(e.w);
+            if (ex == 0) {
+                const int v[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (i + k < n_entries && (v[k] < 0 || v[k] >= n_expert)) {
+                        flag_error(err, kErrBadId);
+                        if (row_of) row_of[i + k] = -1;
+                    }
+            }
+            hit <<= 4 * (lane & 7);  // eight lanes make a word
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) hit |= __shfl_xor_sync(kFull, hit, o);
+            if ((lane & 7) == 0) bits[(j + 4 * tid) >> 5] = hit;
+        }
+        __syncthreads();
+        const int words = ((n + 4 * kRouteThreads - 1) / (4 * kRouteThreads)) * (kRouteThreads / 8);  // written above
+        uint64_t mine = 0;
+        if (2 * tid < words) mine = bits[2 * tid] | (uint64_t)bits[2 * tid + 1] << 32;
+        const int count = __popcll(mine);
+        int inc = count;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(kFull, inc, o);
+            if (lane >= o) inc += y;
+        }
+        const int warp_less = __reduce_add_sync(kFull, less);
+        if (lane == 31) wpre[warp] = inc;
+        if (lane == 0) wless[warp] = warp_less;
+        __syncthreads();
+        const int in_warp = wpre[lane];
+        const int first = __reduce_add_sync(kFull, wless[lane]);                 // entries of smaller experts
+        const int before = __reduce_add_sync(kFull, lane < warp ? in_warp : 0);  // this expert's, in earlier warps
+        const int all = __reduce_add_sync(kFull, in_warp);
+        int row = first + base + before + inc - count;
+        while (mine) {
+            const int i = c0 + 64 * tid + __ffsll((long long)mine) - 1;
+            mine &= mine - 1;
             entries[row] = i;
             if (row_of) row_of[i] = row;
             row++;
-        });
-    if (tid == 0) offsets[ex] = first;
-    if (ex == n_expert - 1 && tid == kRouteThreads - 1) offsets[n_expert] = first + before + inc;
+        }
+        base += all;
+        if (c0 + kRowsChunk >= n_entries && tid == 0) {
+            offsets[ex] = first;
+            if (ex == n_expert - 1) offsets[n_expert] = first + base;
+        }
+        __syncthreads();  // bits and the partial sums are rewritten by the next chunk
+    }
 }
 
 // Self-test of the bounded mbarrier wait: the barrier expects one arrival
@@ -214,10 +249,9 @@ cudaError_t launch_moe_expert_rows(const LaunchCtx &c, const int32_t *idx, int32
                                    int32_t *row_of, int64_t n_entries, int n_expert)
 {
     if (n_expert <= 0 || n_expert > 65535 || n_entries > (1 << 30)) return cudaErrorInvalidValue;
-    const int run = (int)((n_entries + kRouteThreads - 1) / kRouteThreads + 3) & ~3;
     const int vec = (reinterpret_cast<uintptr_t>(idx) & 15u) == 0;
     launch_k(c, moe_expert_rows_k, dim3((unsigned)n_expert), dim3(kRouteThreads), idx, offsets, entries, row_of,
-             (int)n_entries, n_expert, run, vec, c.err);
+             (int)n_entries, n_expert, vec, c.err);
     return cudaGetLastError();
 }
 

@@ -12,18 +12,16 @@ namespace {
 
 // ----------------------------------------------------------------- quantise
 // Rows are dense and a whole number of blocks, so the tensor is a flat list of
-// blocks. A thread converts 8 consecutive elements; the four threads of a
-// block share the largest magnitude by two shuffles. Inputs as for mx_scale:
-// fp16 values convert to fp32 exactly.
-__device__ __forceinline__ void load8(float (&v)[8], const float *p)
+// 16-byte input units (4 fp32 or 8 fp16 elements); the 8 or 4 lanes of a block
+// share the largest magnitude by shuffles. A thread takes kUnits units 256
+// apart, all loads first: every access of a warp is one contiguous run, and
+// the reads in flight cover the latency (98304 x 2048 fp16 to MXFP4 and back:
+// 291 us with one 8-element unit per thread and split accesses).
+constexpr int kUnits = 4;
+
+__device__ __forceinline__ void unpack(float (&v)[4], float4 a) { v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w; }
+__device__ __forceinline__ void unpack(float (&v)[8], float4 a)
 {
-    const float4 a = ld_stream_inflight(reinterpret_cast<const float4 *>(p));
-    const float4 b = ld_stream_inflight(reinterpret_cast<const float4 *>(p) + 1);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-}
-__device__ __forceinline__ void load8(float (&v)[8], const __half *p)
-{
-    const float4 a = ld_stream_inflight(reinterpret_cast<const float4 *>(p));
     const __half2 *h = reinterpret_cast<const __half2 *>(&a);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -34,71 +32,93 @@ __device__ __forceinline__ void load8(float (&v)[8], const __half *p)
 }
 
 template <typename T, bool FP4>
-__global__ void __launch_bounds__(256) mx_quantize_k(const T *src, uint8_t *q, uint8_t *scales, int64_t n8)
+__global__ void __launch_bounds__(256) mx_quantize_k(const T *src, uint8_t *q, uint8_t *scales, int64_t n_units)
 {
+    constexpr int E = 16 / sizeof(T);       // elements per unit
+    constexpr int kLanes = kMxBlock / E;    // lanes per block
     pdl_wait();
     pdl_trigger();
-    const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;  // a block's four threads are in one warp
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (u < n8) load8(v, src + u * 8);
-    uint32_t amax = 0;
+    const int64_t u0 = (int64_t)blockIdx.x * (256 * kUnits) + threadIdx.x;
+    float4 in[kUnits];
 #pragma unroll
-    for (int i = 0; i < 8; i++) amax = max(amax, __float_as_uint(v[i]) & 0x7fffffffu);
-    amax = max(amax, __shfl_xor_sync(kFull, amax, 1));
-    amax = max(amax, __shfl_xor_sync(kFull, amax, 2));
-    if (u >= n8) return;
-    const uint32_t sc = mx_scale<FP4 ? kMxEmaxFp4 : kMxEmaxFp8>(amax);
-    const float inv = mx_inv_scale(sc);
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = mx_scaled(v[i], sc, inv);
-    if (FP4) {
-        *reinterpret_cast<uint32_t *>(q + u * 4) = e2m1x8(v);
-    } else {
-        *reinterpret_cast<uint2 *>(q + u * 8) = make_uint2(e4m3x4(v[0], v[1], v[2], v[3]), e4m3x4(v[4], v[5], v[6], v[7]));
+    for (int k = 0; k < kUnits; k++) {
+        in[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (u0 + 256 * k < n_units) in[k] = ld_stream_inflight(reinterpret_cast<const float4 *>(src) + u0 + 256 * k);
     }
-    if ((threadIdx.x & 3) == 0) scales[u >> 2] = (uint8_t)sc;
+#pragma unroll
+    for (int k = 0; k < kUnits; k++) {
+        float v[E];
+        unpack(v, in[k]);
+        uint32_t amax = 0;
+#pragma unroll
+        for (int i = 0; i < E; i++) amax = max(amax, __float_as_uint(v[i]) & 0x7fffffffu);
+#pragma unroll
+        for (int o = 1; o < kLanes; o <<= 1) amax = max(amax, __shfl_xor_sync(kFull, amax, o));
+        const int64_t u = u0 + 256 * k;
+        if (u >= n_units) continue;  // whole blocks: n is a multiple of 32
+        const uint32_t sc = mx_scale<FP4 ? kMxEmaxFp4 : kMxEmaxFp8>(amax);
+        const float inv = mx_inv_scale(sc);
+#pragma unroll
+        for (int i = 0; i < E; i++) v[i] = mx_scaled(v[i], sc, inv);
+        if constexpr (E == 8) {
+            if (FP4) reinterpret_cast<uint32_t *>(q)[u] = e2m1x8(v);
+            else reinterpret_cast<uint2 *>(q)[u] = make_uint2(e4m3x4(v[0], v[1], v[2], v[3]), e4m3x4(v[4], v[5], v[6], v[7]));
+        } else {
+            if (FP4) {
+                const float w[8] = {v[0], v[1], v[2], v[3], 0.0f, 0.0f, 0.0f, 0.0f};
+                reinterpret_cast<uint16_t *>(q)[u] = (uint16_t)e2m1x8(w);
+            } else {
+                reinterpret_cast<uint32_t *>(q)[u] = e4m3x4(v[0], v[1], v[2], v[3]);
+            }
+        }
+        if (threadIdx.x % kLanes == 0) scales[u / kLanes] = (uint8_t)sc;
+    }
 }
 
 // --------------------------------------------------------------- dequantise
 // Both element types convert to fp16 exactly, and the product with a power of
 // two is exact in fp32 (an element has at most 4 significant bits, so even
-// results below the normal range are representable).
+// results below the normal range are representable). A unit is 4 elements, one
+// 16-byte store; kUnits units per thread as above.
 template <bool FP4>
-__global__ void __launch_bounds__(256) mx_dequantize_k(const uint8_t *q, const uint8_t *scales, float *dst, int64_t n8)
+__global__ void __launch_bounds__(256) mx_dequantize_k(const uint8_t *q, const uint8_t *scales, float *dst, int64_t n_units)
 {
     pdl_wait();
     pdl_trigger();
-    const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (u >= n8) return;
-    uint32_t h[4];
-    if (FP4) {
-        const uint32_t w = __ldcs(reinterpret_cast<const uint32_t *>(q + u * 4));
-        asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-            "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
-            "cvt.rn.f16x2.e2m1x2 %0, b0;\n\tcvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
-            "cvt.rn.f16x2.e2m1x2 %2, b2;\n\tcvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
-            : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
-            : "r"(w));
-    } else {
-        const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(q + u * 8));
-        asm("{\n\t.reg .b16 a, b, c, d;\n\t"
-            "mov.b32 {a, b}, %4;\n\tmov.b32 {c, d}, %5;\n\t"
-            "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t"
-            "cvt.rn.f16x2.e4m3x2 %2, c;\n\tcvt.rn.f16x2.e4m3x2 %3, d;\n\t}"
-            : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
-            : "r"(w.x), "r"(w.y));
-    }
-    const float s = mx_scale_value(scales[u >> 2]);
-    float2 f[4];
+    const int64_t u0 = (int64_t)blockIdx.x * (256 * kUnits) + threadIdx.x;
+    uint32_t w[kUnits], sc[kUnits];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        f[i] = __half22float2(*reinterpret_cast<const __half2 *>(&h[i]));
-        f[i].x *= s;
-        f[i].y *= s;
+    for (int k = 0; k < kUnits; k++) {
+        const int64_t u = u0 + 256 * k;
+        w[k] = sc[k] = 0;
+        if (u < n_units) {
+            w[k] = FP4 ? reinterpret_cast<const uint16_t *>(q)[u] : __ldcs(reinterpret_cast<const uint32_t *>(q) + u);
+            sc[k] = scales[u >> 3];
+        }
     }
-    float4 *o = reinterpret_cast<float4 *>(dst + u * 8);
-    __stcs(o, make_float4(f[0].x, f[0].y, f[1].x, f[1].y));
-    __stcs(o + 1, make_float4(f[2].x, f[2].y, f[3].x, f[3].y));
+#pragma unroll
+    for (int k = 0; k < kUnits; k++) {
+        const int64_t u = u0 + 256 * k;
+        if (u >= n_units) break;
+        uint32_t h[2];
+        if (FP4) {
+            asm("{\n\t.reg .b8 b0, b1;\n\t"
+                "mov.b16 {b0, b1}, %2;\n\t"
+                "cvt.rn.f16x2.e2m1x2 %0, b0;\n\tcvt.rn.f16x2.e2m1x2 %1, b1;\n\t}"
+                : "=&r"(h[0]), "=r"(h[1])
+                : "h"((uint16_t)w[k]));
+        } else {
+            asm("{\n\t.reg .b16 a, b;\n\t"
+                "mov.b32 {a, b}, %2;\n\t"
+                "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+                : "=r"(h[0]), "=r"(h[1])
+                : "r"(w[k]));
+        }
+        const float s = mx_scale_value(sc[k]);
+        const float2 lo = __half22float2(*reinterpret_cast<const __half2 *>(&h[0]));
+        const float2 hi = __half22float2(*reinterpret_cast<const __half2 *>(&h[1]));
+        __stcs(reinterpret_cast<float4 *>(dst) + u, make_float4(lo.x * s, lo.y * s, hi.x * s, hi.y * s));
+    }
 }
 
 // ------------------------------------------------ residual add + norm + MXFP8
@@ -358,32 +378,30 @@ cudaError_t run_norm_mx(const LaunchCtx &c, const float *x, const float *r, cons
 
 cudaError_t launch_mx_quantize(const LaunchCtx &c, const void *src, bool f16, uint8_t *q, uint8_t *scales, int to, int64_t n)
 {
-    const int64_t n8 = n / 8;
-    if (n8 <= 0) return cudaSuccess;
-    const int64_t blocks = (n8 + 255) / 256;
+    const int64_t units = n / (f16 ? 8 : 4), blocks = (units + 256 * kUnits - 1) / (256 * kUnits);
+    if (blocks <= 0) return cudaSuccess;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
     const dim3 g((unsigned)blocks), b(256);
     if (f16) {
         const __half *s = (const __half *)src;
-        if (to == kMxFp4) launch_k(c, mx_quantize_k<__half, true>, g, b, s, q, scales, n8);
-        else launch_k(c, mx_quantize_k<__half, false>, g, b, s, q, scales, n8);
+        if (to == kMxFp4) launch_k(c, mx_quantize_k<__half, true>, g, b, s, q, scales, units);
+        else launch_k(c, mx_quantize_k<__half, false>, g, b, s, q, scales, units);
     } else {
         const float *s = (const float *)src;
-        if (to == kMxFp4) launch_k(c, mx_quantize_k<float, true>, g, b, s, q, scales, n8);
-        else launch_k(c, mx_quantize_k<float, false>, g, b, s, q, scales, n8);
+        if (to == kMxFp4) launch_k(c, mx_quantize_k<float, true>, g, b, s, q, scales, units);
+        else launch_k(c, mx_quantize_k<float, false>, g, b, s, q, scales, units);
     }
     return cudaGetLastError();
 }
 
 cudaError_t launch_mx_dequantize(const LaunchCtx &c, const uint8_t *q, const uint8_t *scales, int from, float *dst, int64_t n)
 {
-    const int64_t n8 = n / 8;
-    if (n8 <= 0) return cudaSuccess;
-    const int64_t blocks = (n8 + 255) / 256;
+    const int64_t units = n / 4, blocks = (units + 256 * kUnits - 1) / (256 * kUnits);
+    if (blocks <= 0) return cudaSuccess;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
     const dim3 g((unsigned)blocks), b(256);
-    if (from == kMxFp4) launch_k(c, mx_dequantize_k<true>, g, b, q, scales, dst, n8);
-    else launch_k(c, mx_dequantize_k<false>, g, b, q, scales, dst, n8);
+    if (from == kMxFp4) launch_k(c, mx_dequantize_k<true>, g, b, q, scales, dst, units);
+    else launch_k(c, mx_dequantize_k<false>, g, b, q, scales, dst, units);
     return cudaGetLastError();
 }
 

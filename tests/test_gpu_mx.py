@@ -233,7 +233,8 @@ def run_rows(ds3, B, idx, E, shift=0):
 
 
 @pytest.mark.parametrize("T,E,K", [(1, 128, 8), (1, 1, 1), (3, 256, 8), (37, 64, 4), (512, 128, 8), (700, 256, 3),
-                                   (5000, 60, 1), (8191, 128, 8)])
+                                   (5000, 60, 1), (8191, 128, 8), (8192, 40, 8), (8193, 40, 8),
+                                   (30000, 250, 5)])
 def test_expert_rows(ds3, B, T, E, K):
     idx = np.argsort(I.rng(T + E).random((T, E)), 1)[:, :K].astype(np.int32)
     rc, got = run_rows(ds3, B, idx, E)
