@@ -105,7 +105,7 @@ struct MoeArgs {
     int n_x, n_rows, n_out_rows, n_group, x_div, K, n_w;
     int x_mode, w_mode;        // how scale rows are loaded (stage_scales)
     unsigned n_mt, n_mt_inv;   // weight blocks per group, 2^32 / n_mt rounded up
-    int half, fp4;             // out is fp16 (2: pairs are aligned); the weights are MXFP4
+    int half, fp4, quads;      // out is fp16; the weights are MXFP4; out rows are whole aligned quads
 };
 
 // ------------------------------------------------------------ PTX wrappers
@@ -127,6 +127,14 @@ __device__ __forceinline__ void tma_load_2d(uint32_t lead, uint32_t dst, const C
         "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
         "@q cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n\t}" ::
             "r"(dst), "l"(m), "r"(x), "r"(y), "r"(bar), "r"(lead) : "memory");
+}
+// The same box into L2 only, a hint.
+__device__ __forceinline__ void tma_prefetch_3d(uint32_t lead, const CUtensorMap *m, int x, int y, int z)
+{
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %4, 0;\n\t"
+        "@q cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];\n\t}" ::
+            "l"(m), "r"(x), "r"(y), "r"(z), "r"(lead) : "memory");
 }
 __device__ __forceinline__ void expect_bytes(uint32_t lead, uint32_t bar, uint32_t bytes)
 {
@@ -257,6 +265,26 @@ __device__ __forceinline__ int x_row(int v, const MoeArgs &a)
     return x < 0 || x >= a.n_x ? 0 : x;
 }
 
+// Four consecutive values of an output row, from column m.
+__device__ __forceinline__ void store4(const MoeArgs &a, size_t at, int m, float4 y)
+{
+    const __half2 lo = __floats2half2_rn(y.x, y.y), hi = __floats2half2_rn(y.z, y.w);
+    if (a.quads && m < a.n_w) {  // rows of whole, aligned quads
+        if (a.half)
+            *reinterpret_cast<uint2 *>(reinterpret_cast<__half *>(a.out) + at) =
+                make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+        else *reinterpret_cast<float4 *>(reinterpret_cast<float *>(a.out) + at) = y;
+        return;
+    }
+    const float f[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if (m + j >= a.n_w) break;
+        if (a.half) reinterpret_cast<__half *>(a.out)[at + j] = __float2half_rn(f[j]);
+        else reinterpret_cast<float *>(a.out)[at + j] = f[j];
+    }
+}
+
 struct Tile {
     int e, mt, n0, rows, r0;  // group, weight block, first row in the group, rows here, first sorted row
 };
@@ -385,7 +413,8 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
     __shared__ __align__(8) uint64_t full[ST], empty[ST], acc_full[2], acc_empty[2], drain;
     __shared__ uint32_t tmem_base;
     __shared__ int n_tiles;
-    __shared__ int wsum[16];
+    __shared__ int wsum[32];
+    __shared__ int tile_rows[8];  // rows of the CTA's tiles, from the warp that stages A's scales
     int *tab = reinterpret_cast<int *>(sm + L::kOffTab);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -432,8 +461,7 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
         }
         if (lane == 31) wsum[warp] = inc;
         __syncthreads();
-        int base = 0;
-        for (int i = 0; i < warp; i++) base += wsum[i];
+        const int base = __reduce_add_sync(kFull, lane < warp ? wsum[lane] : 0);
         // Past the last group v is 0, so the prefix stays at the total there.
         if (tid < kMaxGroups) {
             tab[tid] = lo;
@@ -485,6 +513,14 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
                 }
                 issued++;
                 ring.next();
+                // A CTA with a single tile (decode) has nothing behind it to hide
+                // latency with: once the ring is full, the rest of the tile's
+                // weights are asked into L2 together.
+                if (total <= (int)gridDim.x && kb == ST - 1)
+                    for (int i = ST * L::kSub; i < n_slices; i++) {
+                        tma_prefetch_3d(lead, &maps.w0, i * kSliceK, row, q.e);
+                        if (SWIGLU) tma_prefetch_3d(lead, &maps.w1, i * kSliceK, row, q.e);
+                    }
             }
         }
         if (!ok) {
@@ -513,18 +549,20 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
         const uint64_t bd0 = smem_desc(smem_addr(sm + L::kOffB), 1024, 2);
         const uint64_t sa0 = smem_desc(smem_addr(sm + L::kOffSfA), 128, 0);
         const uint64_t sb0 = smem_desc(smem_addr(sm + L::kOffSfB), 128, 0);
+        bool acc_ready = true;  // a test of acc_empty made ahead of time
         for (int t = blockIdx.x; t < total; t += gridDim.x, it++) {
-            const Tile q = find_tile<NT>(tab, a, t, lane);
             const int b = it & 1;
-            ok = __all_sync(kFull, mbar_wait(&acc_empty[b], ((it >> 1) & 1u) ^ 1u, kWaitLimit));
+            ok = __all_sync(kFull, acc_ready) ||
+                 __all_sync(kFull, mbar_wait(&acc_empty[b], ((it >> 1) & 1u) ^ 1u, kWaitLimit));
             if (!ok) break;
-            tc_fence_after();
-            const uint32_t idesc = idesc0 | ((uint32_t)((q.rows + 15) >> 4) << 18);  // N / 8 at bit 17
+            uint32_t idesc = 0;
             const uint32_t d = tmem + b * NT;
             for (int kb = 0; kb < n_kb; kb++) {
                 ok = ring.wait(full);
                 if (!ok) break;
                 ring.peek(full);
+                if (kb == 0) idesc = idesc0 | ((uint32_t)((*(volatile int *)&tile_rows[it & 7] + 15) >> 4) << 18);  // N / 8 at bit 17
+                if (kb == n_kb - 1) acc_ready = mbar_test(&acc_empty[b ^ 1], (((it + 1) >> 1) & 1u) ^ 1u);
                 const int s = ring.s;
                 tc_fence_after();
                 if (GATHER) fence_async_shared();  // the rows the gathering warps copied
@@ -562,8 +600,14 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
         }
     } else if (warp < 4) {
         // ------------------------------------------------------------ scales
+        int seq = 0;
         auto rows_of_a = [&](const uint8_t *(&row)[4], int t) {
             const Tile q = find_tile<NT>(tab, a, t, lane);
+            // For the issuing warp, which reads it after this tile's first stage.
+            // At most kAhead + ST tiles ahead of it, so eight entries do.
+            static_assert(kAhead + ST < 8, "tile_rows");
+            if (lane == 0) *(volatile int *)&tile_rows[seq & 7] = q.rows;
+            seq++;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int r = min(q.mt * kRowsPerTile + 32 * (SWIGLU ? j & 1 : j) + lane, a.n_w - 1);
@@ -665,41 +709,53 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
         static_assert(NT <= kEpilogueThreads, "one column per epilogue thread");
         float *xch = reinterpret_cast<float *>(sm + L::kOffXch);
         int it = 0, parity = 0;
-        for (int t = blockIdx.x; t < total; t += gridDim.x, it++) {
-            const Tile q = find_tile<NT>(tab, a, t, lane);
-            const int b = it & 1;
-            // While the products run, thread c looks up column c: where its row
-            // goes (-1: nowhere; SwiGLU: its weight) and whether its token row
-            // is one of x. Two buffers: no thread is two tiles ahead of another.
-            int2 *col = reinterpret_cast<int2 *>(sm + L::kOffCol) + b * NT;
-            if (me >= q.rows && me < NT) col[me] = make_int2(-1, 0);
-            if (me < q.rows) {
-                const int r = q.r0 + me;
-                int xid = r;
-                bool good = true;
-                if (a.x_rows) {
-                    xid = a.x_rows[r];
-                    good = xid >= 0 && xid / a.x_div < a.n_x;
-                    if (!good) flag_error(err, kErrBadId);
-                }
-                int to = r;
-                if (SWIGLU) {
-                    to = __float_as_int(a.row_w && good ? a.row_w[xid] : 1.0f);
-                } else if (a.out_rows) {
-                    to = a.out_rows[r];
-                    if (to < 0 || to >= a.n_out_rows) {
-                        to = -1;
-                        flag_error(err, kErrBadId);
-                    }
-                }
-                col[me] = make_int2(to, good);
+        // Thread c looks up column c, a tile ahead: its row's x_rows and out_rows
+        // values when the tile before it begins, its weight when that one's
+        // products are done. (Looked up in its own tile, a memory round trip per
+        // tile was the longest part of a small tile's epilogue.)
+        int next_x = 0, next_o = 0;
+        float next_w = 1.0f;
+        Tile q, next = {};
+        auto look_up = [&](int t) {
+            if (t >= total) return;
+            next = find_tile<NT>(tab, a, t, lane);
+            if (me < next.rows) {
+                const int r = next.r0 + me;
+                next_x = a.x_rows ? a.x_rows[r] : r;
+                next_o = a.out_rows ? a.out_rows[r] : r;
             }
-            // The warps go on together or not at all.
-            ok = named_all(3, kEpilogueThreads, mbar_wait(&acc_full[b], (it >> 1) & 1u, kWaitLimit));
+        };
+        auto good_x = [&](int x) { return !a.x_rows || (x >= 0 && x / a.x_div < a.n_x); };
+        auto look_up_weight = [&] {
+            if (SWIGLU && a.row_w && me < next.rows && good_x(next_x)) next_w = a.row_w[next_x];
+        };
+        look_up(blockIdx.x);
+        look_up_weight();
+        for (int t = blockIdx.x; t < total; t += gridDim.x, it++) {
+            q = next;
+            const int b = it & 1;
+            // Where column c's row goes (-1: nowhere; SwiGLU: its weight) and
+            // whether its token row is one of x. Two buffers: no thread is two
+            // tiles ahead of another.
+            int2 *col = reinterpret_cast<int2 *>(sm + L::kOffCol) + b * NT;
+            if (me < NT) {
+                int2 k = make_int2(-1, 0);
+                if (me < q.rows) {
+                    k.y = good_x(next_x);
+                    k.x = SWIGLU ? __float_as_int(next_w) : next_o >= 0 && next_o < a.n_out_rows ? next_o : -1;
+                    if (!k.y || (!SWIGLU && k.x < 0)) flag_error(err, kErrBadId);
+                }
+                col[me] = k;
+            }
+            look_up(t + gridDim.x);
+            // One warp polls (eight would take issue slots from the others'
+            // work), and all go on together or not at all.
+            ok = named_all(3, kEpilogueThreads, warp != 4 || mbar_wait(&acc_full[b], (it >> 1) & 1u, kWaitLimit));
             if (!ok) {
                 give_up();
                 break;
             }
+            look_up_weight();
             tc_fence_after();
             const uint32_t d = tmem + b * NT + ((uint32_t)(32 * w) << 16);
             // One copy of the chunk's code: with it unrolled over the chunks, the
@@ -722,70 +778,76 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
                     for (int i = 0; i < 8; i++) mine[i * 32 + lane] = __uint_as_float(gate ? v[2 * i + 1] : v[2 * i]);
                     named_sync(4 + side * 2 + (w & 1), 64);
                     const int f0 = q.mt * kRowsPerTile + 32 * (w & 1);
-                    // No branches over the columns, so that the eight run side by
-                    // side: a column alone is 300 cycles of latencies.
-                    float h[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float other = theirs[i * 32 + lane];
-                        const float gv = gate ? __uint_as_float(v[2 * i]) : other;
-                        const float uv = gate ? other : __uint_as_float(v[2 * i + 1]);
-                        const int2 k = col[c0 + 2 * i + (gate ? 0 : 1)];
-                        // silu(g) u: the quotient is good to 2 ulp, far inside the 8-bit rounding.
-                        h[i] = __fdividef(gv, 1.0f + expf(-gv)) * uv;
-                        if (a.row_w) h[i] *= __int_as_float(k.x);
-                        if (!k.y) h[i] = 0.0f;
-                    }
-                    uint32_t sc[8], my_scale = 0;
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        sc[i] = mx_scale<kMxEmaxFp8>(__reduce_max_sync(kFull, __float_as_uint(h[i]) & 0x7fffffffu));
+                    uint32_t my_scale = 0;
                     uint8_t *oq = reinterpret_cast<uint8_t *>(a.out) + (size_t)(q.r0 + c0) * a.n_w + f0 + lane;
+                    // Four columns side by side, without branches between them: a
+                    // column alone is 300 cycles of latencies.
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int c = 2 * i + (gate ? 0 : 1);
-                        const uint32_t e = e4m3x2(mx_scaled(h[i], sc[i], mx_inv_scale(sc[i])), 0.0f);
-                        if (lane == c) my_scale = sc[i];
-                        if (c < nc && f0 < a.n_w) oq[(size_t)c * a.n_w] = (uint8_t)e;
+                    for (int i0 = 0; i0 < 8; i0 += 4) {
+                        if (2 * i0 >= nc) break;
+                        float h[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float other = theirs[(i0 + i) * 32 + lane];
+                            const float gv = gate ? __uint_as_float(v[2 * (i0 + i)]) : other;
+                            const float uv = gate ? other : __uint_as_float(v[2 * (i0 + i) + 1]);
+                            const int2 k = col[c0 + 2 * (i0 + i) + (gate ? 0 : 1)];
+                            // silu(g) u: the quotient is good to 2 ulp, far inside the 8-bit rounding.
+                            h[i] = __fdividef(gv, 1.0f + expf(-gv)) * uv;
+                            if (a.row_w) h[i] *= __int_as_float(k.x);
+                            if (!k.y) h[i] = 0.0f;
+                        }
+                        uint32_t sc[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            sc[i] = mx_scale<kMxEmaxFp8>(__reduce_max_sync(kFull, __float_as_uint(h[i]) & 0x7fffffffu));
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int c = 2 * (i0 + i) + (gate ? 0 : 1);
+                            const uint32_t e = e4m3x2(mx_scaled(h[i], sc[i], mx_inv_scale(sc[i])), 0.0f);
+                            if (lane == c) my_scale = sc[i];
+                            if (c < nc && f0 < a.n_w) oq[(size_t)c * a.n_w] = (uint8_t)e;
+                        }
                     }
                     if ((lane & 1) == (gate ? 0 : 1) && lane < nc && f0 < a.n_w)
                         a.out_s[(size_t)(q.r0 + c0 + lane) * (a.n_w / kMxBlock) + f0 / kMxBlock] = (uint8_t)my_scale;
-                } else {
+                } else if (q.rows <= 16) {
+                    // Few rows: each lane stores its own value of each.
                     const int m = q.mt * kRowsPerTile + 32 * w + lane;
-                    const bool in = m < a.n_w;
-                    // All columns' places first, two to a load; then stores that
-                    // wait for nothing (one by one, a column took 80 cycles).
-                    int4 k[8];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) k[i] = reinterpret_cast<const int4 *>(col + c0)[i];
-                    if (a.half) {
-                        // Two columns at a time: an even lane stores its row and the
-                        // next of the first column, an odd lane of the second.
-                        __half *o = reinterpret_cast<__half *>(a.out);
-                        const int odd = lane & 1;
+                    for (int c = 0; c < 16; c++) {
+                        if (c >= nc) break;
+                        const int2 k = col[c];
+                        if (k.x < 0 || m >= a.n_w) continue;
+                        const size_t at = (size_t)(uint32_t)k.x * (uint32_t)a.n_w + m;
+                        const float y = k.y ? __uint_as_float(v[c]) : 0.0f;
+                        if (a.half) reinterpret_cast<__half *>(a.out)[at] = __float2half_rn(y);
+                        else reinterpret_cast<float *>(a.out)[at] = y;
+                    }
+                } else {
+                    // The side's four warps lay 16 output rows of 128 values side by
+                    // side in shared memory, and each writes four of them whole: one
+                    // 16-byte store per lane and row. (Every warp storing its own 32
+                    // values of each row made the stores the bound: 4096 tokens, 768
+                    // -> 2048, fp16: 119 us against 63 us without an epilogue.)
+                    float *stage = xch + side * 2048;
 #pragma unroll
-                        for (int c = 0; c < 16; c += 2) {
-                            const float v0 = k[c / 2].y ? __uint_as_float(v[c]) : 0.0f;
-                            const float v1 = k[c / 2].w ? __uint_as_float(v[c + 1]) : 0.0f;
-                            const float got = __shfl_xor_sync(kFull, odd ? v0 : v1, 1);
-                            const int to = odd ? k[c / 2].z : k[c / 2].x;
-                            const __half2 pair = odd ? __floats2half2_rn(got, v1) : __floats2half2_rn(v0, got);
-                            __half *at = o + (size_t)(uint32_t)to * (uint32_t)a.n_w + (m - odd);
-                            if (to >= 0 && a.half == 2 && m - odd < a.n_w) {
-                                *reinterpret_cast<__half2 *>(at) = pair;
-                            } else if (to >= 0) {  // rows of an odd length, or an odd base
-                                if (m - odd < a.n_w) at[0] = __low2half(pair);
-                                if (m - odd + 1 < a.n_w) at[1] = __high2half(pair);
-                            }
-                        }
-                    } else {
-                        float *o = reinterpret_cast<float *>(a.out) + m;
+                    for (int c = 0; c < 16; c++) stage[c * 128 + 32 * w + lane] = __uint_as_float(v[c]);
+                    named_sync(4 + side, 128);
+                    const int m = q.mt * kRowsPerTile + 4 * lane;
+                    float4 y[4];
+                    int2 k[4];
 #pragma unroll
-                        for (int c = 0; c < 16; c++) {
-                            const int to = c & 1 ? k[c / 2].z : k[c / 2].x, good = c & 1 ? k[c / 2].w : k[c / 2].y;
-                            if (to >= 0 && in)
-                                o[(size_t)(uint32_t)to * (uint32_t)a.n_w] = good ? __uint_as_float(v[c]) : 0.0f;
-                        }
+                    for (int i = 0; i < 4; i++) {
+                        y[i] = *reinterpret_cast<const float4 *>(stage + (4 * w + i) * 128 + 4 * lane);
+                        k[i] = col[c0 + 4 * w + i];
+                    }
+                    named_sync(4 + side, 128);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        if (k[i].x < 0) continue;
+                        if (!k[i].y) y[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        store4(a, (size_t)(uint32_t)k[i].x * (uint32_t)a.n_w + m, m, y[i]);
                     }
                 }
             }
@@ -910,8 +972,8 @@ cudaError_t launch_moe_mx(const LaunchCtx &c, const MoeMxCall &q)
     MoeArgs a = {};
     a.x = q.x;
     a.x_s = q.x_s;
-    // Pairs of an fp16 row are whole words when the row length is even and the base aligned.
-    a.half = !q.out_f16 ? 0 : q.n_w % 2 == 0 && (uintptr_t)q.out % 4 == 0 ? 2 : 1;
+    a.half = q.out_f16;
+    a.quads = q.n_w % 4 == 0 && (uintptr_t)q.out % (q.out_f16 ? 8 : 16) == 0;
     a.fp4 = fp4;
     a.w0_s = q.w0_s;
     a.w1_s = q.w1_s;
