@@ -780,14 +780,16 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
                     const int f0 = q.mt * kRowsPerTile + 32 * (w & 1);
                     uint32_t my_scale = 0;
                     uint8_t *oq = reinterpret_cast<uint8_t *>(a.out) + (size_t)(q.r0 + c0) * a.n_w + f0 + lane;
-                    // Four columns side by side, without branches between them: a
-                    // column alone is 300 cycles of latencies.
+                    // Columns side by side, without branches between them: a column
+                    // alone is 300 cycles of latencies. Eight at a time for wide
+                    // tiles, four where most tiles have fewer rows.
+                    constexpr int kSide = NT == 64 ? 4 : 8;
 #pragma unroll
-                    for (int i0 = 0; i0 < 8; i0 += 4) {
+                    for (int i0 = 0; i0 < 8; i0 += kSide) {
                         if (2 * i0 >= nc) break;
-                        float h[4];
+                        float h[kSide];
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
+                        for (int i = 0; i < kSide; i++) {
                             const float other = theirs[(i0 + i) * 32 + lane];
                             const float gv = gate ? __uint_as_float(v[2 * (i0 + i)]) : other;
                             const float uv = gate ? other : __uint_as_float(v[2 * (i0 + i) + 1]);
@@ -797,12 +799,12 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
                             if (a.row_w) h[i] *= __int_as_float(k.x);
                             if (!k.y) h[i] = 0.0f;
                         }
-                        uint32_t sc[4];
+                        uint32_t sc[kSide];
 #pragma unroll
-                        for (int i = 0; i < 4; i++)
+                        for (int i = 0; i < kSide; i++)
                             sc[i] = mx_scale<kMxEmaxFp8>(__reduce_max_sync(kFull, __float_as_uint(h[i]) & 0x7fffffffu));
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
+                        for (int i = 0; i < kSide; i++) {
                             const int c = 2 * (i0 + i) + (gate ? 0 : 1);
                             const uint32_t e = e4m3x2(mx_scaled(h[i], sc[i], mx_inv_scale(sc[i])), 0.0f);
                             if (lane == c) my_scale = sc[i];
@@ -811,13 +813,14 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
                     }
                     if ((lane & 1) == (gate ? 0 : 1) && lane < nc && f0 < a.n_w)
                         a.out_s[(size_t)(q.r0 + c0 + lane) * (a.n_w / kMxBlock) + f0 / kMxBlock] = (uint8_t)my_scale;
-                } else if (q.rows <= 16) {
-                    // Few rows: each lane stores its own value of each.
+                } else if (NT == 64) {
+                    // Few rows: each lane stores its own value of each. (Staged as
+                    // below: 16 tokens 19.1 against 17.5 us, 512 tokens alike.)
                     const int m = q.mt * kRowsPerTile + 32 * w + lane;
 #pragma unroll
                     for (int c = 0; c < 16; c++) {
                         if (c >= nc) break;
-                        const int2 k = col[c];
+                        const int2 k = col[c0 + c];
                         if (k.x < 0 || m >= a.n_w) continue;
                         const size_t at = (size_t)(uint32_t)k.x * (uint32_t)a.n_w + m;
                         const float y = k.y ? __uint_as_float(v[c]) : 0.0f;
