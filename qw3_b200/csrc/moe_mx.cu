@@ -228,9 +228,9 @@ __device__ __forceinline__ void tc_ld16(uint32_t (&v)[16], uint32_t tmem)
         : "r"(tmem)
         : "memory");
 }
-// Between shared-memory writes by threads and the tensor core's reads of them:
-// by the writer before it arrives (scales; its warp has the time), or, for rows
-// whose copies land after their thread has gone on, by the issuing warp.
+// Between shared-memory writes by threads (scales, gathered rows), seen through
+// a barrier, and the tensor core's reads of them: in the issuing warp. In the
+// scale warps it would also wait for their loads ahead (a DRAM latency per tile).
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // Whether `ok` holds in all `threads` threads that meet at barrier `id`.
 __device__ __forceinline__ bool named_all(int id, int threads, bool ok)
@@ -318,9 +318,12 @@ __device__ __forceinline__ Tile find_tile(const int *tab, const MoeArgs &a, int 
 // their use in registers: MODE 2, all words of a row and stage at once (K a
 // whole number of stages); 1, word by word (K % 128 == 0); 0, words put
 // together from bytes (other K, an odd base).
-// Copying each word asynchronously to its place instead cost 52 cycles of
-// issue per copy and bounded the small tiles (512 tokens, 768 -> 2048: 33 us).
-constexpr int kAhead = 3;
+// The ring of stages hides most of the latency, and every buffer more is one
+// more copy of the loop: the roles' code competes for the instruction caches,
+// and kAhead 1 / 3 / 7 took 152 / 164 / 170 us (4096 tokens, 2048 -> 2 x 768)
+// and 30 / 31 / 38 us (16 tokens, MXFP4). Copying each word asynchronously to
+// its place cost 52 cycles of issue per copy.
+constexpr int kAhead = 1;
 
 __device__ __forceinline__ void ld_word(uint32_t &v, const uint8_t *p)
 {
@@ -384,7 +387,6 @@ __device__ __forceinline__ bool stage_scales(Rows &rows_of, uint8_t *dst, uint64
                         *reinterpret_cast<uint4 *>(dst + ring.s * BYTES + i * (BYTES / SUB) + j * 128 + lane * 16) =
                             make_uint4(w(0), w(1), w(2), w(3));
                     }
-                fence_async_shared();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[ring.s]);
                 ring.next();
@@ -565,7 +567,7 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
                 if (kb == n_kb - 1) acc_ready = mbar_test(&acc_empty[b ^ 1], (((it + 1) >> 1) & 1u) ^ 1u);
                 const int s = ring.s;
                 tc_fence_after();
-                if (GATHER) fence_async_shared();  // the rows the gathering warps copied
+                fence_async_shared();
                 // Scales of the slices side by side: A's 4 columns, then B's.
                 const uint32_t sf = tmem + 2 * NT + s * L::kSfCols;
 #pragma unroll
@@ -780,10 +782,9 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
                     const int f0 = q.mt * kRowsPerTile + 32 * (w & 1);
                     uint32_t my_scale = 0;
                     uint8_t *oq = reinterpret_cast<uint8_t *>(a.out) + (size_t)(q.r0 + c0) * a.n_w + f0 + lane;
-                    // Columns side by side, without branches between them: a column
-                    // alone is 300 cycles of latencies. Eight at a time for wide
-                    // tiles, four where most tiles have fewer rows.
-                    constexpr int kSide = NT == 64 ? 4 : 8;
+                    // Four columns side by side, without branches between them: a
+                    // column alone is 300 cycles of latencies.
+                    constexpr int kSide = 4;
 #pragma unroll
                     for (int i0 = 0; i0 < 8; i0 += kSide) {
                         if (2 * i0 >= nc) break;
