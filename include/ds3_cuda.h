@@ -443,10 +443,15 @@ int ds3_cuda_moe_expert_rows(const ds3_cuda_buffer_t *idx, ds3_cuda_buffer_t *of
  * w_type. out: fp32 or fp16 rows of n_out (out_type); o(r) = out_rows[r]
  * (int32 [n_rows]; entries puts results back in token order), or r when
  * out_rows is NULL. Sums are fp32. n_in % 32 == 0 for MXFP8 weights, % 128 ==
- * 0 for MXFP4. A row of x named outside [0, n_x) gives a zero row, an output
- * row outside `out` is skipped, a bad offsets table is clamped; each makes the
- * call return -1. With n_expert 1 and offsets {0, n_rows} it is a dense
- * product. n_expert <= 256. */
+ * 0 for MXFP4. out_rows must not name a row twice. A row of x named outside
+ * [0, n_x) gives a zero row, an output row outside `out` is skipped, bounds
+ * outside [0, n_rows] are clamped, and offsets that decrease anywhere leave
+ * `out` as it was; each makes the call return -1. With n_expert 1 and offsets
+ * {0, n_rows} it is a dense product. n_expert <= 256.
+ * With x_rows and more than 48 rows per expert on average, the rows are first
+ * sorted into the library's workspace (n_rows * n_in * 33/32 bytes, allocated
+ * on first use and kept). Where it cannot grow (inside a graph capture, or no
+ * memory) the product gathers them itself: same results, slower. */
 int ds3_cuda_moe_mx_matmul(const ds3_cuda_buffer_t *x_q, const ds3_cuda_buffer_t *x_scales,
                            const ds3_cuda_buffer_t *x_rows, uint32_t x_div, const ds3_cuda_buffer_t *offsets,
                            const ds3_cuda_buffer_t *w_q, const ds3_cuda_buffer_t *w_scales, ds3_cuda_mx_t w_type,

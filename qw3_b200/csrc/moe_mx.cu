@@ -35,11 +35,18 @@
 //     through a shared-memory exchange, and a warp's 32 lanes are the 32
 //     elements of one MX block.
 //
-// Warps: 0 copies (weights: tiled boxes; token rows: tiled boxes when
-// they are used in place), 1 issues the tensor-
-// core work, 2 / 3 stage the scales of A / B in the order the tensor core
-// wants them (row r of 128 -> lane r%32, word r/32), 4-11 are the epilogue,
-// and 12-15 gather token rows that come through x_rows.
+// Warps: 0 copies (weights, and token rows that are used in place, as tiled
+// boxes), 1 issues the tensor-core work, 2 / 3 stage the scales of A / B in the
+// order the tensor core wants them (row r of 128 -> lane r%32, word r/32), 4-11
+// are the epilogue, and 12-15 gather token rows that come through x_rows.
+//
+// What bounds it (B200, 6.5 TB/s measured copy rate). Up to about 128 rows per
+// expert the weights' HBM bytes: 512 tokens x top-8 of 128 experts, 2048 -> 2 x
+// 768: MXFP8 5.5 TB/s. MXFP4 halves the bytes, and then the issuing warp's and
+// the copy engine's work per stage bounds it (3.7 TB/s). Long batches: the
+// operands' way from L2 to the SMs (about 10.7 TB/s there) and power: 4096
+// tokens, 1.35 PFLOP/s in place at full clocks.
+//
 // Every wait is bounded; on a timeout the CTA records it, lets its copies and
 // products land (bounded), frees its tensor memory and returns.
 #include "common.cuh"
@@ -441,16 +448,20 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
     pdl_wait();
     pdl_trigger();
 
-    // Group bounds, clamped to 0 <= off[e] <= off[e+1] <= n_rows (a bad table
-    // is reported and never read past), and the tile prefix.
+    // Group bounds, clamped to [0, n_rows], and the tile prefix. A table that
+    // decreases anywhere means nothing: no group has rows then (groups would
+    // overlap, and their tiles outnumber any bound). Either is reported.
     {
-        int lo = 0, hi = 0;
+        int lo = 0, hi = 0, l0 = 0, h0 = 0;
         if (tid < a.n_group) {
-            const int l0 = a.offsets[tid], h0 = a.offsets[tid + 1];
+            l0 = a.offsets[tid];
+            h0 = a.offsets[tid + 1];
             lo = min(max(l0, 0), a.n_rows);
-            hi = min(max(h0, lo), a.n_rows);
-            if ((lo != l0 || hi != h0) && blockIdx.x == 0) flag_error(err, kErrBadId);
+            hi = min(max(h0, 0), a.n_rows);
         }
+        const bool decreases = __syncthreads_or(h0 < l0);
+        if ((lo != l0 || hi != h0 || decreases) && blockIdx.x == 0) flag_error(err, kErrBadId);
+        if (decreases) hi = lo;
         // A group's token blocks are of one size, a multiple of 16 (at most NT,
         // so that the last one is never empty).
         const int blocks = (hi - lo + NT - 1) / NT;

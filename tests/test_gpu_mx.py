@@ -400,6 +400,10 @@ def test_matmul_bad_maps_and_offsets(ds3, B):
         want = R.grouped(xd, wd, np.array(good), src)
         want[good[-1]:] = 5.0
         assert_bitexact(got, want.astype(np.float32), "clamped")
+    for table in ([0, 30, 20], [40, 0, 40], [9, 8, 7]):  # decreasing: nothing is written
+        rc, got = run_matmul(ds3, B, x, xs, w, ws, FP8, np.array(table, np.int32), 40,
+                             np.full((40, 64), 5.0, np.float32), src)
+        assert rc == -1 and (got == 5.0).all()
     # a good call after them succeeds
     rc, _ = run_matmul(ds3, B, x, xs, w, ws, FP8, off, 40, np.zeros((40, 64), np.float32), src)
     assert rc == 0
@@ -470,6 +474,38 @@ def test_matmul_unaligned_scales_and_offsets_past_32_bits(ds3, B):
     assert ds3.moe_mx_matmul(B.up(x), B.up(xs), None, 1, B.up(off), big, bigs, FP8, o, F32, None, rows, rows, E, K, N2) == 0
     got = B.down(o, np.float32, (rows, N2))[:, -N:]
     assert_bitexact(got, want.astype(np.float32), "far end")
+
+
+@pytest.mark.parametrize("rows,E,K,N", [(2000, 30, 640, 900), (3000, 14, 768, 2000), (6000, 12, 1024, 1500)])
+def test_matmul_gathers_where_the_workspace_cannot_grow(ds3, B, rows, E, K, N):
+    """A capture before any workspace exists: wide tiles gather their rows in
+    the kernel. The same call outside sorts them first; both are exact."""
+    ds3.shutdown()
+    assert ds3.init() == 0
+    x, xs = exact_rows(1, rows // 2, K, FP8)
+    w, ws = exact_rows(2, E * N, K, FP8)
+    off = ragged(3, rows, E, 0.1)
+    src = I.rng(4).integers(0, rows // 2, rows).astype(np.int32)
+    b = [B.up(v) for v in (x, xs, src, off, w, ws)]
+    outs = [B.up(np.full((rows, N), np.nan, np.float32)) for _ in range(2)]
+    call = lambda o: ds3.moe_mx_matmul(b[0], b[1], b[2], 1, b[3], b[4], b[5], FP8, o, F32, None, rows // 2, rows,  # noqa: E731
+                                       E, K, N)
+    assert ds3.graph_begin() == 0
+    rc = call(outs[0])
+    g = ds3.graph_end()
+    assert rc == 0, ds3.last_error()
+    assert ds3.graph_launch(g) == 0
+    ds3.synchronize()
+    assert call(outs[1]) == 0
+    want = R.grouped(R.decode(x, xs, FP8), R.decode(w, ws, FP8).reshape(E, N, K), off, src).astype(np.float32)
+    for o in outs:
+        assert_bitexact(B.down(o, np.float32, (rows, N)), want, "out")
+    # replayed again after the workspace exists
+    assert ds3.buffer_write(outs[0], 0, np.zeros((rows, N), np.float32)) == 0
+    assert ds3.graph_launch(g) == 0
+    ds3.synchronize()
+    ds3.graph_free(g)
+    assert_bitexact(B.down(outs[0], np.float32, (rows, N)), want, "replayed")
 
 
 # -------------------------------------------------------------------- SwiGLU
