@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(256) mx_dequantize_k(const uint8_t *q, const u
 // x and of r per thread, all loads issued before the first use), so the reads
 // and writes of other rows pass under a row's reductions. Thread t works on
 // elements 4 t .. 4 t + 3 of every 512: an MX block is 8 neighbouring lanes.
-// 16384 x 2048: 95 us, 6.0 TB/s; without the prefetch of the next wave's rows
+// 16384 x 2048: 93 us, 6.2 TB/s; without the prefetch of the next wave's rows
 // 103 us; with one warp per row and the row in shared memory, the first
 // version, 149 us (too few reads in flight behind its chains).
 // Longer rows: that version, below.
@@ -186,9 +186,12 @@ __device__ __forceinline__ double sumsq4(float4 v, double acc)
     return fma((double)v.w, (double)v.w, acc);
 }
 
-template <int VPT>
-__global__ void __launch_bounds__(128, VPT <= 4 ? 8 : 4) add_rms_norm_mx_row(const float *x, const float *r, const float *w, float *sum_out,
-                                                           float *norm_out, uint8_t *q, uint8_t *scales, int n, int ahead, float eps)
+// FEW: one wave of rows at most. Registers are free then, and the norm weight
+// (a parameter the operation just before must not write) is loaded before the
+// programmatic-launch wait, which takes a round trip out of the chain.
+template <int VPT, bool FEW>
+__global__ void __launch_bounds__(128, FEW ? 1 : VPT <= 4 ? 8 : 4) add_rms_norm_mx_row(const float *x, const float *r, const float *w, float *sum_out,
+                                                           float *norm_out, uint8_t *q, uint8_t *scales, int n, double inv_n, int ahead, float eps)
 {
     __shared__ double part[4];
     const int tid = threadIdx.x, n4 = n / 4;
@@ -200,10 +203,16 @@ __global__ void __launch_bounds__(128, VPT <= 4 ? 8 : 4) add_rms_norm_mx_row(con
         if (tid < 2 && p) prefetch_l2(p + at * n, (uint64_t)n * 4);
     };
     if (row < ahead) prefetch(row);
+    const float4 *xr = reinterpret_cast<const float4 *>(x + row * n), *w4 = reinterpret_cast<const float4 *>(w);
+    float4 wv[FEW ? VPT : 1];
+    if (FEW) {
+#pragma unroll
+        for (int i = 0; i < VPT; i++)
+            if (tid + 128 * i < n4) wv[FEW ? i : 0] = ld_param(w4 + tid + 128 * i);
+    }
     pdl_wait();
     pdl_trigger();
-    if (row + ahead < gridDim.x) prefetch(row + ahead);
-    const float4 *xr = reinterpret_cast<const float4 *>(x + row * n), *w4 = reinterpret_cast<const float4 *>(w);
+    if (!FEW && row + ahead < gridDim.x) prefetch(row + ahead);
     float4 v[VPT];
 #pragma unroll
     for (int i = 0; i < VPT; i++) {
@@ -235,7 +244,7 @@ __global__ void __launch_bounds__(128, VPT <= 4 ? 8 : 4) add_rms_norm_mx_row(con
     if ((tid & 31) == 0) part[tid >> 5] = ss;
     __syncthreads();
     ss = (part[0] + part[1]) + (part[2] + part[3]);
-    const double inv = inv_sqrt64(ss / (double)n + (double)eps);
+    const double inv = inv_sqrt64(fma(ss, inv_n, (double)eps));
     const float ih = (float)inv, il = (float)(inv - (double)ih);
     float4 *no = norm_out ? reinterpret_cast<float4 *>(norm_out + row * n) : nullptr;
     uint32_t *qo = reinterpret_cast<uint32_t *>(q + row * n);
@@ -245,7 +254,7 @@ __global__ void __launch_bounds__(128, VPT <= 4 ? 8 : 4) add_rms_norm_mx_row(con
     for (int i = 0; i < VPT; i++) {
         const int c = tid + 128 * i;
         if (c < n4) {
-            v[i] = norm4(v[i], inv, ih, il, ld_param(w4 + c));
+            v[i] = norm4(v[i], inv, ih, il, FEW ? wv[FEW ? i : 0] : ld_param(w4 + c));
             if (no) no[c] = v[i];
         }
         amax[i] = amax4(v[i]);
@@ -419,10 +428,17 @@ cudaError_t launch_add_rms_norm_mx(const LaunchCtx &c, const float *x, const flo
         if (rows > 0x7fffffffLL) return cudaErrorInvalidValue;
         const dim3 g((unsigned)rows), b(128);
         const int ahead = c.n_sm * 8;  // about one wave of rows
-        if (n <= 512) launch_k(c, add_rms_norm_mx_row<1>, g, b, x, r, w, sum_out, norm_out, q, scales, n, ahead, eps);
-        else if (n <= 1024) launch_k(c, add_rms_norm_mx_row<2>, g, b, x, r, w, sum_out, norm_out, q, scales, n, ahead, eps);
-        else if (n <= 2048) launch_k(c, add_rms_norm_mx_row<4>, g, b, x, r, w, sum_out, norm_out, q, scales, n, ahead, eps);
-        else launch_k(c, add_rms_norm_mx_row<8>, g, b, x, r, w, sum_out, norm_out, q, scales, n, ahead, eps);
+        const double inv_n = 1.0 / n;
+#define DS3_NORM(VPT)                                                                                                  \
+    (rows <= ahead ? launch_k(c, add_rms_norm_mx_row<VPT, true>, g, b, x, r, w, sum_out, norm_out, q, scales, n, inv_n, \
+                              ahead, eps)                                                                              \
+                   : launch_k(c, add_rms_norm_mx_row<VPT, false>, g, b, x, r, w, sum_out, norm_out, q, scales, n,      \
+                              inv_n, ahead, eps))
+        if (n <= 512) DS3_NORM(1);
+        else if (n <= 1024) DS3_NORM(2);
+        else if (n <= 2048) DS3_NORM(4);
+        else DS3_NORM(8);
+#undef DS3_NORM
         return cudaGetLastError();
     }
     // Two rows in flight per warp when a warp has more than one and they fit.
