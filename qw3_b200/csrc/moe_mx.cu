@@ -321,17 +321,15 @@ __device__ __forceinline__ Tile find_tile(const int *tab, const MoeArgs &a, int 
 // One warp stages the scales of J x 32 operand rows for every stage of every
 // tile of this CTA. Lane l owns rows l, l + 32, ...; the four scales of a row
 // and slice are one word, and the words of the lane's rows lie side by side,
-// which is the tensor core's order. They are loaded kAhead stages ahead of
-// their use in registers: MODE 2, all words of a row and stage at once (K a
-// whole number of stages); 1, word by word (K % 128 == 0); 0, words put
-// together from bytes (other K, an odd base).
-// The ring of stages hides most of the latency, and every buffer more is one
-// more copy of the loop: the roles' code competes for the instruction caches,
-// and kAhead 1 / 3 / 7 took 152 / 164 / 170 us (4096 tokens, 2048 -> 2 x 768)
-// and 30 / 31 / 38 us (16 tokens, MXFP4). Copying each word asynchronously to
-// its place cost 52 cycles of issue per copy.
-constexpr int kAhead = 1;
-
+// which is the tensor core's order. A stage's words are loaded one stage ahead.
+// MODE 2, all words of a row and stage at once (K a whole
+// number of stages); 1, word by word (K % 128 == 0); 0, words put together from
+// bytes (other K, an odd base).
+// The loop is kept rolled: the roles' code competes for the instruction caches,
+// and an unrolled loop with buffers for 3 / 7 stages ahead took 164 / 170 us
+// against 152 (4096 tokens, 2048 -> 2 x 768) and 31 / 38 against 29 (16 tokens,
+// MXFP4). Copying each word asynchronously to its place cost 52 cycles of issue
+// per copy.
 __device__ __forceinline__ void ld_word(uint32_t &v, const uint8_t *p)
 {
     asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p));
@@ -346,12 +344,9 @@ __device__ __forceinline__ bool stage_scales(Rows &rows_of, uint8_t *dst, uint64
                                              int n_kb, int nk32, int lane)
 {
     const uint8_t *row[J];
-    uint32_t buf[kAhead + 1][J][SUB];
-    int lt = blockIdx.x, lkb = 0;  // load cursor: tile, stage
-    auto load = [&](uint32_t (&v)[J][SUB]) {
-        if (lt >= total) return;
-        if (lkb == 0) rows_of(row, lt);
-        const int k = 4 * SUB * lkb;  // first scale of the stage
+    uint32_t cur[J][SUB], nxt[J][SUB];
+    auto load = [&](uint32_t (&v)[J][SUB], int kb) {
+        const int k = 4 * SUB * kb;  // first scale of the stage
 #pragma unroll
         for (int j = 0; j < J; j++) {
             if (MODE == 2 && SUB == 2) {
@@ -370,38 +365,38 @@ __device__ __forceinline__ bool stage_scales(Rows &rows_of, uint8_t *dst, uint64
                 }
             }
         }
-        if (++lkb == n_kb) {
-            lkb = 0;
-            lt += gridDim.x;
-        }
     };
     Ring<ST> ring(1u);
-    int t = blockIdx.x, kb = 0;
-#pragma unroll
-    for (int u = 0; u < kAhead; u++) load(buf[u]);
-    while (t < total) {
-#pragma unroll
-        for (int u = 0; u <= kAhead; u++) {
-            load(buf[(u + kAhead) % (kAhead + 1)]);
-            if (t < total) {
-                if (!ring.wait(empty)) return false;
-                ring.peek(empty);
-#pragma unroll
-                for (int i = 0; i < SUB; i++)
-#pragma unroll
-                    for (int j = 0; j < J; j += 4) {
-                        auto w = [&](int n) { return j + n < J ? buf[u][j + n < J ? j + n : 0][i] : 0u; };
-                        *reinterpret_cast<uint4 *>(dst + ring.s * BYTES + i * (BYTES / SUB) + j * 128 + lane * 16) =
-                            make_uint4(w(0), w(1), w(2), w(3));
-                    }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&full[ring.s]);
-                ring.next();
-                if (++kb == n_kb) {
-                    kb = 0;
-                    t += gridDim.x;
-                }
+    if ((int)blockIdx.x < total) {
+        rows_of(row, blockIdx.x);
+        load(cur, 0);
+    }
+    for (int t = blockIdx.x; t < total; t += gridDim.x) {
+#pragma unroll 1
+        for (int kb = 0; kb < n_kb; kb++) {
+            if (kb + 1 < n_kb) {
+                load(nxt, kb + 1);
+            } else if (t + (int)gridDim.x < total) {
+                rows_of(row, t + gridDim.x);
+                load(nxt, 0);
             }
+            if (!ring.wait(empty)) return false;
+            ring.peek(empty);
+#pragma unroll
+            for (int i = 0; i < SUB; i++)
+#pragma unroll
+                for (int j = 0; j < J; j += 4) {
+                    auto w = [&](int n) { return j + n < J ? cur[j + n < J ? j + n : 0][i] : 0u; };
+                    *reinterpret_cast<uint4 *>(dst + ring.s * BYTES + i * (BYTES / SUB) + j * 128 + lane * 16) =
+                        make_uint4(w(0), w(1), w(2), w(3));
+                }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[ring.s]);
+            ring.next();
+#pragma unroll
+            for (int j = 0; j < J; j++)
+#pragma unroll
+                for (int i = 0; i < SUB; i++) cur[j][i] = nxt[j][i];
         }
     }
     return true;
@@ -617,8 +612,8 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
         auto rows_of_a = [&](const uint8_t *(&row)[4], int t) {
             const Tile q = find_tile<NT>(tab, a, t, lane);
             // For the issuing warp, which reads it after this tile's first stage.
-            // At most kAhead + ST tiles ahead of it, so eight entries do.
-            static_assert(kAhead + ST < 8, "tile_rows");
+            // At most ST + 1 tiles ahead of it, so eight entries do.
+            static_assert(ST + 1 < 8, "tile_rows");
             if (lane == 0) *(volatile int *)&tile_rows[seq & 7] = q.rows;
             seq++;
 #pragma unroll
