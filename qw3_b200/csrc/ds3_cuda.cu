@@ -1415,7 +1415,8 @@ int ds3_cuda_moe_expert_rows(const ds3_cuda_buffer_t *idx, ds3_cuda_buffer_t *of
     if (!need(op, "idx", idx, ent) || !need(op, "offsets", offsets, ob) || !writable(op, "offsets", offsets) ||
         !need(op, "entries", entries, ent) || !writable(op, "entries", entries) ||
         (row_of && (!need(op, "row_of", row_of, ent) || !writable(op, "row_of", row_of))) ||
-        !disjoint(op, "offsets", offsets, ob, "idx", idx, ent) || !disjoint(op, "entries", entries, ent, "idx", idx, ent) ||
+        !aligned(op, "idx", idx, 4) || !aligned(op, "offsets", offsets, 4) || !aligned(op, "entries", entries, 4) ||
+        !aligned(op, "row_of", row_of, 4) || !disjoint(op, "offsets", offsets, ob, "idx", idx, ent) || !disjoint(op, "entries", entries, ent, "idx", idx, ent) ||
         !disjoint(op, "row_of", row_of, ent, "idx", idx, ent) ||
         !disjoint(op, "entries", entries, ent, "offsets", offsets, ob) ||
         !disjoint(op, "row_of", row_of, ent, "offsets", offsets, ob) ||

@@ -122,6 +122,13 @@ def test_expert_rows_refusals(buf, change, word):
     refused(ds3.moe_expert_rows(*a.values()), word)
 
 
+@pytest.mark.parametrize("which", ["idx", "offsets", "entries", "row_of"])
+def test_expert_rows_refuses_odd_addresses(buf, which):
+    a = dict(idx=buf(128), offsets=buf(65 * 4), entries=buf(128), row_of=buf(128), n_tokens=4, n_expert=64, n_used=8)
+    a[which] = buf(65 * 4, 2)
+    refused(ds3.moe_expert_rows(*a.values()), "4-byte aligned")
+
+
 def matmul(buf, **k):
     # 4 experts, 8 rows, 256 -> 96
     a = dict(x_q=buf(8 * 256), x_scales=buf(64), x_rows=buf(32), x_div=1, offsets=buf(20), w_q=buf(4 * 96 * 256),
