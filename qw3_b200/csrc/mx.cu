@@ -154,16 +154,22 @@ __device__ __forceinline__ float4 norm4(float4 s, double inv, float ih, float il
 {
     const float a[4] = {__fmul_rn(s.x, ih), __fmul_rn(s.y, ih), __fmul_rn(s.z, ih), __fmul_rn(s.w, ih)};
     const float low = fminf(fminf(fabsf(a[0]), fabsf(a[1])), fminf(fabsf(a[2]), fabsf(a[3])));
-    // Below 2^-100 the carried errors would leave fp32's range: products in fp64.
-    if (inv < 0x1p-100 || low < 0x1p-100f)
-        return make_float4((float)((double)s.x * inv * (double)g.x), (float)((double)s.y * inv * (double)g.y),
-                           (float)((double)s.z * inv * (double)g.z), (float)((double)s.w * inv * (double)g.w));
+    // Below 2^-100 the carried errors would leave fp32's range: products in fp64, as behind.
+    bool wide = inv < 0x1p-100 || low < 0x1p-100f;
     auto one = [&](float x, float a, float g) {
         const float ae = fmaf(x, il, fmaf(x, ih, -a));
         const float h = __fmul_rn(a, g);
         return __fadd_rn(h, fmaf(ae, g, fmaf(a, g, -h)));
     };
-    return make_float4(one(s.x, a[0], g.x), one(s.y, a[1], g.y), one(s.z, a[2], g.z), one(s.w, a[3], g.w));
+    const float4 y = make_float4(one(s.x, a[0], g.x), one(s.y, a[1], g.y), one(s.z, a[2], g.z), one(s.w, a[3], g.w));
+    // A factor or a value past fp32's range leaves a NaN here (inf - inf), and
+    // so do NaN inputs: fp64 tells them apart. (NaN in any makes the sum NaN.)
+    const float sum = (y.x + y.y) + (y.z + y.w);
+    wide |= sum != sum;
+    if (wide)
+        return make_float4((float)((double)s.x * inv * (double)g.x), (float)((double)s.y * inv * (double)g.y),
+                           (float)((double)s.z * inv * (double)g.z), (float)((double)s.w * inv * (double)g.w));
+    return y;
 }
 
 __device__ __forceinline__ uint32_t amax4(float4 v)

@@ -198,6 +198,27 @@ def test_norm_extreme_rows(ds3, B):
     check_norm(x, None, w, 1e-6, run_norm(ds3, B, x, None, w))
 
 
+@pytest.mark.parametrize("n", [128, 8224])
+def test_norm_factors_out_of_range(ds3, B, n):
+    """An inverse root past fp32's range (subnormal rows, eps 0) and weights
+    that carry normed values past it: the exact value rounded once, infinite
+    where that is."""
+    x, w = I.normal(1, (3, n)), I.gamma(n, 3)
+    x[1] *= np.float32(1e-40)
+    w[64] = 3e38
+    got = run_norm(ds3, B, x, None, w, eps=0.0)
+    _, wn = R.add_norm(x, None, w, 0.0)
+    with np.errstate(over="ignore"):
+        want = wn.astype(np.float32)
+    assert np.isinf(want[:, 64]).any() and np.isfinite(np.delete(want, 64, 1)).all()
+    fin = np.isfinite(want)
+    assert (got[1][~fin] == want[~fin]).all(), "infinities"
+    assert (np.abs(got[1] - wn)[fin] <= np.abs(wn[fin]) * 2.0**-24 * (1 + 2.0**-18) + 2.0**-150).all()
+    wq, ws = R.encode(want, FP8)
+    assert_bitexact(got[3], ws, "scales")
+    assert_bitexact(got[2], wq, "elements")
+
+
 @pytest.mark.parametrize("bad", [np.inf, np.nan])
 def test_norm_nonfinite_row(ds3, B, bad):
     """As the plain formula: an infinity makes its own place NaN and the rest
