@@ -801,8 +801,11 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
                             const float gv = gate ? __uint_as_float(v[2 * (i0 + i)]) : other;
                             const float uv = gate ? other : __uint_as_float(v[2 * (i0 + i) + 1]);
                             const int2 k = col[c0 + 2 * (i0 + i) + (gate ? 0 : 1)];
-                            // silu(g) u: the quotient is good to 2 ulp, far inside the 8-bit rounding.
-                            h[i] = __fdividef(gv, 1.0f + expf(-gv)) * uv;
+                            // silu(g) u. With e^-|g| the divisor is 1 to 2 for every gate, where
+                            // the quotient is good to 2 ulp, far inside the 8-bit rounding. (It is
+                            // 0 for divisors past 2^126, that of e^-g below -87.3.)
+                            const float t = expf(-fabsf(gv));
+                            h[i] = __fdividef(gv < 0.0f ? gv * t : gv, 1.0f + t) * uv;
                             if (a.row_w) h[i] *= __int_as_float(k.x);
                             if (!k.y) h[i] = 0.0f;
                         }

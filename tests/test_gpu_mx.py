@@ -8,7 +8,7 @@ sum is a whole number of quanta below 2^24), which leaves no tolerance for a
 misplaced row, column, block or scale; on ordinary values each product carries
 at most one rounding per term, K 2^-23 sum|x w|. SwiGLU's 8-bit result is off
 the exact value by half an element step, plus the fp32 chain before it: expf
-and the quotient 2 ulp each, three more roundings, under 8 * 2^-24 * 2 in all.
+and the quotient 2 ulp each, four more roundings, under 8 * 2^-24 * 2 in all.
 """
 
 from __future__ import annotations
@@ -602,6 +602,36 @@ def test_swiglu_bad_rows_and_large_gates(ds3, B):
     gate = xd[rows[ok]] @ gd.T
     assert np.abs(gate).max() > 500
     check_act(got_q[ok], got_s[ok], R.silu(gate) * (xd[rows[ok]] @ ud.T))
+
+
+def test_swiglu_gates_where_the_exponential_leaves_the_normal_range(ds3, B):
+    """silu(-87.5) is 1e-36 and comes back into range with a large up product.
+    The exponential there is a whole number of 2^-149: two of them are its
+    2 ulp, times gate and up."""
+    gates = [-80.0, -87.5, -88.0, 88.0]
+    K, F, rows = 128, 32 * len(gates), 3
+    one = np.zeros((rows, K))
+    one[:, :2] = 1.0
+    x, xs = R.encode(one, FP8)
+    g = np.zeros((F, K))
+    for i, v in enumerate(gates):
+        big = np.sign(v) * 80.0 if abs(v) % 8 else v  # the sum of two e4m3 values
+        g[32 * i:32 * i + 32, 0], g[32 * i:32 * i + 32, 1] = big, v - big
+    # the two terms have to survive one scale
+    gq, gs = R.encode(g, FP8)
+    gd = R.decode(gq, gs, FP8)
+    assert (gd == g).all()
+    u = np.zeros((F, K))
+    u[:, 0] = 2.0**120
+    u *= np.where(np.arange(F) % 2, 1.0, -1.5)[:, None]
+    uq, us = R.encode(u, FP8)
+    assert (R.decode(uq, us, FP8) == u).all()
+    q, s = B.up(np.zeros((rows, F), np.uint8)), B.up(np.zeros((rows, F // 32), np.uint8))
+    assert ds3.moe_mx_swiglu(B.up(x), B.up(xs), None, 1, B.up(np.array([0, rows], np.int32)), B.up(gq), B.up(gs), B.up(uq),
+                             B.up(us), FP8, None, q, s, rows, rows, 1, K, F) == 0, ds3.last_error()
+    gate, up = one @ g.T, one @ u.T
+    slack = np.where(gate < 0, 2 * 2.0**-149 * np.abs(gate * up), 0.0)
+    check_act(B.down(q, np.uint8, (rows, F)), B.down(s, np.uint8, (rows, F // 32)), R.silu(gate) * up, slack)
 
 
 # ------------------------------------------------------------- the whole path
