@@ -448,10 +448,11 @@ int ds3_cuda_moe_expert_rows(const ds3_cuda_buffer_t *idx, ds3_cuda_buffer_t *of
  * outside [0, n_rows] are clamped, and offsets that decrease anywhere leave
  * `out` as it was; each makes the call return -1. With n_expert 1 and offsets
  * {0, n_rows} it is a dense product. n_expert <= 256.
- * With x_rows and more than 48 rows per expert on average, the rows are first
- * sorted into the library's workspace (n_rows * n_in * 33/32 bytes, allocated
- * on first use and kept). Where it cannot grow (inside a graph capture, or no
- * memory) the product gathers them itself: same results, slower. */
+ * With x_rows and more than 96 rows per expert on average (48 for MXFP4
+ * weights), the rows are first sorted into the library's workspace (n_rows *
+ * n_in * 33/32 bytes, allocated on first use and kept). Where it cannot grow
+ * (inside a graph capture, or no memory) the product gathers them itself: same
+ * results, slower. */
 int ds3_cuda_moe_mx_matmul(const ds3_cuda_buffer_t *x_q, const ds3_cuda_buffer_t *x_scales,
                            const ds3_cuda_buffer_t *x_rows, uint32_t x_div, const ds3_cuda_buffer_t *offsets,
                            const ds3_cuda_buffer_t *w_q, const ds3_cuda_buffer_t *w_scales, ds3_cuda_mx_t w_type,
