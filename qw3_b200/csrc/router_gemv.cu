@@ -84,15 +84,6 @@ struct AddNorm {
     int w_early;      // W is a weight no preceding op writes: its copy may start before the PDL wait
 };
 
-__device__ __forceinline__ uint32_t cluster_rank()
-{
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_arrive_release() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
-__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait_acquire() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 // Store one float into the shared memory of CTA `rank` of this cluster, at the
 // offset `local` has in this CTA.
 __device__ __forceinline__ void st_cluster_f32(const float *local, uint32_t rank, float v)

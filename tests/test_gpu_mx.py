@@ -287,6 +287,27 @@ def test_expert_rows_bad_ids(ds3, B):
     assert_bitexact(row, w_row)
 
 
+@pytest.mark.parametrize("n", [28 * 1024, 28 * 1024 + 1, 65536, 65537, 200003])
+def test_expert_rows_many_entries_bad_ids_unaligned(ds3, B, n):
+    """Sizes on both sides of the switch to clusters and of their chunks, ids
+    out of range either way, and expert counts that leave a cluster part-filled."""
+    idx = I.rng(n).integers(0, 19, (n, 1)).astype(np.int32)
+    idx[[0, n // 2, n - 1]] = np.array([[19], [-1], [-(1 << 31)]], np.int32)
+    idx[5::7] = 18  # a popular last expert
+    rc, (off, ent, row) = run_rows(ds3, B, idx, 19, shift=4)
+    assert rc == -1
+    w_off, w_ent, w_row = R.expert_rows(idx, 19)
+    assert_bitexact(off, w_off)
+    assert_bitexact(ent[: len(w_ent)], w_ent)
+    assert (ent[len(w_ent):] == -7).all()
+    assert_bitexact(row, w_row)
+    ib = B.up(np.full((n, 1), 3, np.int32))  # all to one, no map
+    off, ent = B.up(np.zeros(10, np.int32)), B.up(np.zeros(n, np.int32))
+    assert ds3.moe_expert_rows(ib, off, ent, None, n, 9, 1) == 0, ds3.last_error()
+    assert_bitexact(B.down(off, np.int32, (10,)), np.array([0] * 4 + [n] * 6, np.int32))
+    assert_bitexact(B.down(ent, np.int32, (n,)), np.arange(n, dtype=np.int32))
+
+
 def test_expert_rows_no_tokens(ds3, B):
     off = B.up(np.full(5, 9, np.int32))
     e = B.up(np.zeros(4, np.int32))
