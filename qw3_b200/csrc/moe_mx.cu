@@ -112,7 +112,7 @@ struct MoeArgs {
     int n_x, n_rows, n_out_rows, n_group, x_div, K, n_w;
     int x_mode, w_mode;        // how scale rows are loaded (stage_scales)
     unsigned n_mt, n_mt_inv;   // weight blocks per group, 2^32 / n_mt rounded up
-    int half, fp4, quads;      // out is fp16; the weights are MXFP4; out rows are whole aligned quads
+    int half, fp4, units;      // out is fp16; the weights are MXFP4; out rows are whole aligned 16-byte units
 };
 
 // ------------------------------------------------------------ PTX wrappers
@@ -272,24 +272,14 @@ __device__ __forceinline__ int x_row(int v, const MoeArgs &a)
     return x < 0 || x >= a.n_x ? 0 : x;
 }
 
-// Four consecutive values of an output row, from column m.
-__device__ __forceinline__ void store4(const MoeArgs &a, size_t at, int m, float4 y)
+// 16 bytes of the output row that k names, from column m of `size`-byte values:
+// nothing for a row that goes nowhere, zeros where its token row is none of x.
+__device__ __forceinline__ void store16(const MoeArgs &a, int2 k, int m, uint4 y, uint32_t size)
 {
-    const __half2 lo = __floats2half2_rn(y.x, y.y), hi = __floats2half2_rn(y.z, y.w);
-    if (a.quads && m < a.n_w) {  // rows of whole, aligned quads
-        if (a.half)
-            *reinterpret_cast<uint2 *>(reinterpret_cast<__half *>(a.out) + at) =
-                make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
-        else *reinterpret_cast<float4 *>(reinterpret_cast<float *>(a.out) + at) = y;
-        return;
-    }
-    const float f[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        if (m + j >= a.n_w) break;
-        if (a.half) reinterpret_cast<__half *>(a.out)[at + j] = __float2half_rn(f[j]);
-        else reinterpret_cast<float *>(a.out)[at + j] = f[j];
-    }
+    if (!k.y) y = make_uint4(0, 0, 0, 0);
+    if (k.x >= 0 && m < a.n_w)
+        *reinterpret_cast<uint4 *>(reinterpret_cast<uint8_t *>(a.out) +
+                                   ((size_t)(uint32_t)k.x * (uint32_t)a.n_w + m) * size) = y;
 }
 
 struct Tile {
@@ -823,9 +813,46 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
                     }
                     if ((lane & 1) == (gate ? 0 : 1) && lane < nc && f0 < a.n_w)
                         a.out_s[(size_t)(q.r0 + c0 + lane) * (a.n_w / kMxBlock) + f0 / kMxBlock] = (uint8_t)my_scale;
-                } else if (NT == 64) {
-                    // Few rows: each lane stores its own value of each. (Staged as
-                    // below: 16 tokens 19.1 against 17.5 us, 512 tokens alike.)
+                } else if (a.units) {
+                    // Output rows of whole 16-byte units: the side's four warps lay
+                    // rows of 128 values side by side in shared memory, 4 KB at a
+                    // time in two buffers in turn (so one barrier each), and store
+                    // them whole, 16 bytes a lane. What counts is the number of
+                    // accesses: 4096 tokens, 768 -> 2048, fp16, 79 us, against 96 us
+                    // with 8 bytes a lane, 119 us with every warp storing its own 32
+                    // values of each row, and 68 us without an epilogue.
+                    uint8_t *stage = reinterpret_cast<uint8_t *>(xch) + side * 8192;
+                    const int m0 = q.mt * kRowsPerTile;
+                    if (a.half) {
+                        __half *h = reinterpret_cast<__half *>(stage + parity * 4096);
+                        parity ^= 1;
+#pragma unroll
+                        for (int c = 0; c < 16; c++) h[c * 128 + 32 * w + lane] = __float2half_rn(__uint_as_float(v[c]));
+                        named_sync(4 + side, 128);
+                        const int m = 8 * (lane & 15);
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {  // two rows per store
+                            const int r = 4 * w + 2 * i + (lane >> 4);
+                            store16(a, col[c0 + r], m0 + m, *reinterpret_cast<const uint4 *>(h + r * 128 + m), 2);
+                        }
+                    } else {
+#pragma unroll
+                        for (int half = 0; half < 2; half++) {
+                            if (8 * half >= nc) break;
+                            float *f = reinterpret_cast<float *>(stage + parity * 4096);
+                            parity ^= 1;
+#pragma unroll
+                            for (int c = 0; c < 8; c++) f[c * 128 + 32 * w + lane] = __uint_as_float(v[8 * half + c]);
+                            named_sync(4 + side, 128);
+#pragma unroll
+                            for (int i = 0; i < 2; i++) {
+                                const int r = 2 * w + i;
+                                store16(a, col[c0 + 8 * half + r], m0 + 4 * lane,
+                                        *reinterpret_cast<const uint4 *>(f + r * 128 + 4 * lane), 4);
+                            }
+                        }
+                    }
+                } else {  // each lane stores its own value of each row
                     const int m = q.mt * kRowsPerTile + 32 * w + lane;
 #pragma unroll
                     for (int c = 0; c < 16; c++) {
@@ -836,31 +863,6 @@ __global__ void __launch_bounds__(moe_threads(GATHER), 1) moe_mx_k(const __grid_
                         const float y = k.y ? __uint_as_float(v[c]) : 0.0f;
                         if (a.half) reinterpret_cast<__half *>(a.out)[at] = __float2half_rn(y);
                         else reinterpret_cast<float *>(a.out)[at] = y;
-                    }
-                } else {
-                    // The side's four warps lay 16 output rows of 128 values side by
-                    // side in shared memory, and each writes four of them whole: one
-                    // 16-byte store per lane and row. (Every warp storing its own 32
-                    // values of each row made the stores the bound: 4096 tokens, 768
-                    // -> 2048, fp16: 119 us against 63 us without an epilogue.)
-                    float *stage = xch + side * 2048;
-#pragma unroll
-                    for (int c = 0; c < 16; c++) stage[c * 128 + 32 * w + lane] = __uint_as_float(v[c]);
-                    named_sync(4 + side, 128);
-                    const int m = q.mt * kRowsPerTile + 4 * lane;
-                    float4 y[4];
-                    int2 k[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        y[i] = *reinterpret_cast<const float4 *>(stage + (4 * w + i) * 128 + 4 * lane);
-                        k[i] = col[c0 + 4 * w + i];
-                    }
-                    named_sync(4 + side, 128);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        if (k[i].x < 0) continue;
-                        if (!k[i].y) y[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        store4(a, (size_t)(uint32_t)k[i].x * (uint32_t)a.n_w + m, m, y[i]);
                     }
                 }
             }
@@ -988,7 +990,7 @@ cudaError_t launch_moe_mx(const LaunchCtx &c, const MoeMxCall &q)
     a.x = q.x;
     a.x_s = q.x_s;
     a.half = q.out_f16;
-    a.quads = q.n_w % 4 == 0 && (uintptr_t)q.out % (q.out_f16 ? 8 : 16) == 0;
+    a.units = (size_t)q.n_w * (q.out_f16 ? 2 : 4) % 16 == 0 && (uintptr_t)q.out % 16 == 0;
     a.fp4 = fp4;
     a.w0_s = q.w0_s;
     a.w1_s = q.w1_s;

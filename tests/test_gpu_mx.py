@@ -396,6 +396,33 @@ def test_matmul_many_tiles_per_cta(ds3, B, rows, E, K, N, mapped):
     assert_bitexact(got, want.astype(np.float32), "out")
 
 
+@pytest.mark.parametrize("rows,E", [(900, 20), (1500, 16), (3000, 12)])
+@pytest.mark.parametrize("N", [1000, 1004, 1001])
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("shift", [0, 8])
+def test_matmul_output_units(ds3, B, rows, E, N, dtype, shift):
+    """Every way of storing output rows: whole 16-byte units of either type, and
+    rows whose length or address is not a whole number of them; rows in any
+    order, an x row out of range (zeros) and an output row out of range."""
+    K = 256
+    x, xs = exact_rows(1, rows, K, FP8)
+    w, ws = exact_rows(2, E * N, K, FP4)
+    off = ragged(3, rows, E, 0.1)
+    g = I.rng(4)
+    x_rows, out_rows = g.permutation(rows).astype(np.int32), g.permutation(rows).astype(np.int32)
+    bad_x, bad_o = off[-1] // 2, off[-1] // 3
+    x_rows[bad_x], out_rows[bad_o] = rows, -1
+    out = np.full((rows, N), -77.0, dtype)
+    ob = B.shifted(out, shift) if shift else B.up(out)
+    assert ds3.moe_mx_matmul(B.up(x), B.up(xs), B.up(x_rows), 1, B.up(off), B.up(w), B.up(ws), FP4, ob,
+                             F16 if dtype == np.float16 else F32, B.up(out_rows), rows, rows, E, K, N) == -1
+    y = R.grouped(R.decode(x, xs, FP8), R.decode(w, ws, FP4).reshape(E, N, K), off, np.where(x_rows < rows, x_rows, 0))
+    y[bad_x] = 0.0
+    live = np.setdiff1d(np.arange(off[-1]), [bad_o])
+    out[out_rows[live]] = y[live].astype(np.float32).astype(dtype)
+    assert_bitexact(B.down(ob, dtype, (rows, N)), out, "out")
+
+
 def test_matmul_rows_behind_the_last_group_are_left(ds3, B):
     x, xs = exact_rows(1, 40, 128, FP8)
     w, ws = exact_rows(2, 2 * 64, 128, FP8)
