@@ -1488,7 +1488,7 @@ static int moe_mx_common(const char *op, const ds3_cuda_buffer_t *x_q, const ds3
     }
     const uintptr_t wa = w_type == DS3_CUDA_MXFP4 ? 32 : 16;
     if (!aligned(op, "x_q", x_q, 16) || !aligned(op, swiglu ? "gate_q" : "w_q", w0, wa) || !aligned(op, "up_q", w1, wa) ||
-        !aligned(op, on, out, es) || !aligned(op, "offsets", offsets, 4) || !aligned(op, "x_rows", x_rows, 4) ||
+        !aligned(op, on, out, swiglu ? 16 : es) || !aligned(op, "offsets", offsets, 4) || !aligned(op, "x_rows", x_rows, 4) ||
         !aligned(op, "out_rows", out_rows, 4) || !aligned(op, "row_weight", row_weight, 4))
         return -1;
     const struct {

@@ -189,6 +189,10 @@ def test_swiglu_refusals(buf, change, word):
     refused(swiglu(buf, **change), word)
 
 
+def test_swiglu_refuses_unaligned_rows(buf):
+    refused(swiglu(buf, act_q=buf(16 * 96, 4)), "16-byte aligned")
+
+
 def test_good_arguments_reach_the_device_check(buf):
     import torch
 
