@@ -42,10 +42,10 @@
 //
 // What bounds it (B200, 6.5 TB/s measured copy rate). Up to about 128 rows per
 // expert the weights' HBM bytes: 512 tokens x top-8 of 128 experts, 2048 -> 2 x
-// 768: MXFP8 5.5 TB/s. MXFP4 halves the bytes, and then the issuing warp's and
-// the copy engine's work per stage bounds it (3.7 TB/s). Long batches: the
+// 768: MXFP8 5.6 TB/s. MXFP4 halves the bytes, and then the issuing warp's and
+// the copy engine's work per stage bounds it (4.3 TB/s). Long batches: the
 // operands' way from L2 to the SMs (about 10 TB/s there) and power: 4096
-// tokens, 1.27 PFLOP/s in place.
+// tokens, 1.35 PFLOP/s in place. The epilogue then counts too (20 of 150 us).
 //
 // Every wait is bounded; on a timeout the CTA records it, lets its copies and
 // products land (bounded), frees its tensor memory and returns.
@@ -970,9 +970,9 @@ static int moe_mean_rows(int n_rows, int n_group) { return (n_rows + n_group - 1
 // Gathering inside the product kernel goes through the threads' copy path,
 // which cannot feed wide tiles; sorting the rows first costs a pass over them.
 // Measured, 128 groups, 2048 -> 2 x 768, us gathered / sorted first: MXFP8
-// weights, mean 32 rows 74 / 80, 64: 80 / 87, 80: 85 / 91, 96: 92 / 95, 112:
-// 99 / 97, 128: 119 / 110; MXFP4, whose weights hide less of it, 32: 51 / 55,
-// 64: 68 / 67, 80: 76 / 72, 96: 84 / 75, 128: 118 / 95.
+// weights, mean 32 rows 74 / 79, 64: 80 / 85, 80: 83 / 90, 96: 90 / 93, 112:
+// 97 / 95, 128: 118 / 107; MXFP4, whose weights hide less of it, 32: 50 / 53,
+// 64: 67 / 65, 80: 74 / 70, 96: 82 / 72, 128: 118 / 91.
 size_t moe_sort_bytes(const MoeMxCall &q)
 {
     if (!q.x_rows || moe_mean_rows(q.n_rows, q.n_group) <= (q.w_type == kMxFp4 ? 48 : 96)) return 0;
@@ -1026,9 +1026,10 @@ cudaError_t launch_moe_mx(const LaunchCtx &c, const MoeMxCall &q)
         !encode(&maps.x, a.x, 2, q.K, n_map, 1, 32, false))
         return cudaErrorInvalidValue;
     // Token columns per tile by the groups' mean size. Measured over 128 groups,
-    // 2048 -> 2 x 768, MXFP8, us at 64 / 128 / 224 columns: mean 32: 73 / 74 /
-    // 81, 64: 82 / 77 / 86, 96: 102 / 84 / 91, 128: 123 / 102 / 98, 256: 207 /
-    // 162 / 162. (Groups of about 128 rows mostly need a second block of 128.)
+    // 2048 -> 2 x 768, MXFP8, us at 64 / 128 / 224 columns: mean 32: 71 / 73 /
+    // 80, 48: 74 / 74 / 82, 64: 80 / 76 / 84, 96: 100 / 82 / 89, 128: 119 / 99 /
+    // 96, 256: 200 / 157 / 158. (Half of the groups of about 128 rows need a
+    // second block of 128.)
     const int avg = moe_mean_rows(q.n_rows, q.n_group);
     const int nt = avg <= 48 ? 64 : avg <= 112 ? 128 : 224;
 #define DS3_MOE(NT)                                                                                                  \
