@@ -447,7 +447,7 @@ int ds3_cuda_moe_expert_rows(const ds3_cuda_buffer_t *idx, ds3_cuda_buffer_t *of
  * [0, n_x) gives a zero row, an output row outside `out` is skipped, bounds
  * outside [0, n_rows] are clamped, and offsets that decrease anywhere leave
  * `out` as it was; each makes the call return -1. With n_expert 1 and offsets
- * {0, n_rows} it is a dense product. n_expert <= 256.
+ * {0, n_rows} it is a dense product. n_expert <= 256, n_rows <= 2^30.
  * With x_rows and more than 96 rows per expert on average (48 for MXFP4
  * weights), the rows are first sorted into the library's workspace (n_rows *
  * n_in * 33/32 bytes, allocated on first use and kept). Where it cannot grow

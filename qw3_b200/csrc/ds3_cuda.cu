@@ -1448,9 +1448,13 @@ static int moe_mx_common(const char *op, const ds3_cuda_buffer_t *x_q, const ds3
         set_error("%s: x_div must be > 0", op);
         return -1;
     }
-    if (n_x > 0x7fffffffu || n_rows > 0x7fffffffu || n_in > (1u << 24) || n_out > (1u << 24) ||
-        (x_rows && (uint64_t)n_x * x_div > 0x7fffffffu)) {
-        set_error("%s: n_x, n_rows or n_x * x_div exceeds 2^31 - 1, or n_in or the row length 2^24", op);
+    // The kernel rounds row counts up to whole blocks in 32 bits: 2^30, as moe_expert_rows, leaves room.
+    if (n_rows > (1u << 30)) {
+        set_error("%s: n_rows %u exceeds 2^30", op, n_rows);
+        return -1;
+    }
+    if (n_x > 0x7fffffffu || n_in > (1u << 24) || n_out > (1u << 24) || (x_rows && (uint64_t)n_x * x_div > 0x7fffffffu)) {
+        set_error("%s: n_x or n_x * x_div exceeds 2^31 - 1, or n_in or the row length 2^24", op);
         return -1;
     }
     const uint32_t k_step = w_type == DS3_CUDA_MXFP4 ? 128 : 32;

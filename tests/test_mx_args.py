@@ -200,3 +200,31 @@ def test_good_arguments_reach_the_device_check(buf):
         pytest.skip("a GPU is present: these addresses must not be launched on")
     for rc in (quantize(buf), norm(buf), matmul(buf), swiglu(buf)):
         refused(rc, "not initialised")
+
+
+def many_rows(op, mapped, n):
+    """n rows of 32 elements, with buffers that would hold them."""
+    at = iter(range(1 << 43, 1 << 47, 1 << 43))
+    huge = lambda: ds3.buffer_wrap(next(at), 1 << 42)  # noqa: E731
+    a = dict(x_q=huge(), x_scales=huge(), x_rows=huge() if mapped else None, x_div=1, n_x=n, n_rows=n, n_expert=1, n_in=32)
+    a.update(dict(out=huge(), out_type=F16, n_out=1) if op is matmul else
+             dict(act_q=huge(), act_scales=huge(), row_weight=None, n_ff=32))
+    return op(Arena(), **a)
+
+
+@pytest.mark.parametrize("n", [(1 << 30) + 1, (1 << 31) - 223, (1 << 31) - 1])
+@pytest.mark.parametrize("mapped", [False, True])
+@pytest.mark.parametrize("op", [matmul, swiglu])
+def test_products_refuse_more_than_2_30_rows(op, mapped, n):
+    """Near 2^31 the kernels' counts of row blocks would leave 31 bits."""
+    refused(many_rows(op, mapped, n), "2^30")
+
+
+@pytest.mark.parametrize("mapped", [False, True])
+@pytest.mark.parametrize("op", [matmul, swiglu])
+def test_products_take_2_30_rows(op, mapped):
+    import torch
+
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is present: these addresses must not be launched on")
+    refused(many_rows(op, mapped, 1 << 30), "not initialised")
