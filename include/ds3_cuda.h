@@ -324,7 +324,8 @@ int ds3_cuda_add_rms_norm_router_topk(const ds3_cuda_buffer_t *x, const ds3_cuda
  * (the GGUF nb[1]); input fp32 [n_embd]; gate_logits fp32 [n_expert]. A
  * weight other than dense F32 is converted to fp32 in a library-owned
  * device workspace first (n_expert * n_embd * 4 bytes, allocated on first
- * use and kept): make the first such call outside a graph capture. */
+ * use, kept, and shared with the products further below): make the first such
+ * call outside a graph capture. */
 int ds3_cuda_moe_ffn_router(const ds3_cuda_buffer_t *input, const ds3_cuda_buffer_t *w_gate_inp,
                             ds3_cuda_buffer_t *gate_logits, uint32_t n_embd, uint32_t n_expert,
                             uint64_t router_row_stride, ds3_type_t router_type);
@@ -450,9 +451,12 @@ int ds3_cuda_moe_expert_rows(const ds3_cuda_buffer_t *idx, ds3_cuda_buffer_t *of
  * {0, n_rows} it is a dense product. n_expert <= 256, n_rows <= 2^30.
  * With x_rows and more than 96 rows per expert on average (48 for MXFP4
  * weights), the rows are first sorted into the library's workspace (n_rows *
- * n_in * 33/32 bytes, allocated on first use and kept). Where it cannot grow
- * (inside a graph capture, or no memory) the product gathers them itself: same
- * results, slower. */
+ * n_in * 33/32 bytes). It is allocated on first use, grows to at least twice its
+ * size when a call needs more, and is kept until shutdown: up to twice the
+ * largest request, and as much again where graphs captured smaller blocks.
+ * Where it cannot grow (inside a graph capture, or no memory) the product
+ * gathers the rows itself: same results, slower. Products that could run at the
+ * same time (graphs replayed on streams other than the module's) race on it. */
 int ds3_cuda_moe_mx_matmul(const ds3_cuda_buffer_t *x_q, const ds3_cuda_buffer_t *x_scales,
                            const ds3_cuda_buffer_t *x_rows, uint32_t x_div, const ds3_cuda_buffer_t *offsets,
                            const ds3_cuda_buffer_t *w_q, const ds3_cuda_buffer_t *w_scales, ds3_cuda_mx_t w_type,

@@ -56,11 +56,15 @@ struct State {
     bool pdl = true;  // DS3_CUDA_PDL=0 disables programmatic dependent launch
     // Library-owned device workspace: the fp32 copy of a router matrix stored
     // in another type (moe_ffn_router*), sorted token rows (moe_mx_*). Every use
-    // is written and read by consecutive launches on the one stream. Earlier, smaller allocations stay
-    // alive until shutdown: graphs captured before a growth still use them.
+    // is written and read by consecutive launches on the one stream. A smaller
+    // block before it stays alive until shutdown where a graph captured its
+    // use (graphs may still replay it), and is freed otherwise.
     float *ws = nullptr;
     size_t ws_bytes = 0;
+    bool ws_captured = false;      // a capture used `ws`
     std::vector<void *> ws_old;
+    size_t ws_refused = 0;         // an optional block of this size did not fit,
+    unsigned ws_skipped = 0;       // and so many calls went without since
     std::vector<cudaEvent_t> timers;
     std::vector<cudaEvent_t> event_pool;
     std::vector<ProfileRec> prof;
@@ -191,27 +195,59 @@ int finish(const char *op, cudaError_t launch, ProfScope &ps)
     return sync_and_check(op);
 }
 
+// Whether the module stream is being captured, by graph_begin or by its host.
+bool stream_captured()
+{
+    if (G.capturing) return true;
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    return cudaStreamIsCapturing(G.stream, &st) == cudaSuccess && st != cudaStreamCaptureStatusNone;
+}
+
 // At least `bytes` of library workspace, or nullptr (error set, unless the
 // caller does not `need` it). It only grows outside a graph capture (an
-// allocation cannot be captured).
+// allocation cannot be captured), to twice its size or more: scratch follows
+// the batch, and a batch that grows token by token must not leave a block per
+// size behind. All blocks together, captured ones included, are then under
+// twice the last one, and that one under twice the largest request.
 float *workspace(const char *op, size_t bytes, bool need = true)
 {
-    if (G.ws_bytes >= bytes) return G.ws;
-    if (G.capturing) {
-        set_error("%s: the library workspace needs %zu bytes; make this call once outside a graph capture first",
-                  op, bytes);
+    const bool captured = stream_captured();
+    if (G.ws_bytes >= bytes) {
+        G.ws_captured |= captured;
+        return G.ws;
+    }
+    if (captured) {
+        if (need)
+            set_error("%s: the library workspace needs %zu bytes; make this call once outside a graph capture first",
+                      op, bytes);
         return nullptr;
     }
+    // A failed allocation is slow: who can go without tries such a size again every 64th time.
+    if (!need && G.ws_refused && bytes >= G.ws_refused && ++G.ws_skipped % 64) return nullptr;
+    size_t size = bytes > 2 * G.ws_bytes ? bytes : 2 * G.ws_bytes;
     void *p = nullptr;
-    const cudaError_t e = cudaMalloc(&p, bytes);
+    cudaError_t e = cudaMalloc(&p, size);
+    if (e != cudaSuccess && size > bytes) {
+        cudaGetLastError();
+        size = bytes;
+        e = cudaMalloc(&p, size);
+    }
     if (e != cudaSuccess) {
+        cudaGetLastError();
         if (need) set_error("%s: workspace of %zu bytes: %s", op, bytes, cudaGetErrorString(e));
-        else cudaGetLastError();
+        else G.ws_refused = bytes;
         return nullptr;
     }
-    if (G.ws) G.ws_old.push_back(G.ws);
+    G.ws_refused = 0;
+    if (G.ws_captured) {
+        G.ws_old.push_back(G.ws);
+    } else if (G.ws) {
+        cudaStreamSynchronize(G.stream);  // a batch's launches before this one may use it
+        cudaFree(G.ws);
+    }
     G.ws = (float *)p;
-    G.ws_bytes = bytes;
+    G.ws_bytes = size;
+    G.ws_captured = false;
     return G.ws;
 }
 
@@ -1537,7 +1573,7 @@ static int moe_mx_common(const char *op, const ds3_cuda_buffer_t *x_q, const ds3
     // Scratch for sorted rows, when there is or can be enough: inside a capture
     // it does not grow, and a failed allocation only means the slower gather.
     const size_t scratch = ds3::moe_sort_bytes(c);
-    if (scratch && (G.ws_bytes >= scratch || !G.capturing)) c.sorted = (uint8_t *)workspace(op, scratch, false);
+    if (scratch) c.sorted = (uint8_t *)workspace(op, scratch, false);
     ProfScope ps(op);
     return finish(op, ds3::launch_moe_mx(ctx(), c), ps);
 }

@@ -791,3 +791,117 @@ def test_layer_graph_replay_on_new_inputs(ds3, B, fmt):
                     assert_bitexact(v, e[k], k)
     finally:
         ds3.graph_free(g)
+
+
+# ------------------------------------------------------------- the workspace
+class Sorted:
+    """A product over mapped rows that are sorted into the workspace first, with exact operands."""
+
+    def __init__(self, ds3, B, seed, K=2048, N=32, n_x=64):
+        self.d, self.B, self.K, self.N = ds3, B, K, N
+        self.x, self.xs = exact_rows(seed, n_x, K, FP8)
+        w, ws = exact_rows(seed + 1, N, K, FP8)
+        self.wd = R.decode(w, ws, FP8)
+        self.b = [B.up(v) for v in (self.x, self.xs, w, ws)]
+
+    def call(self, out, rows, off, n):
+        x, xs, w, ws = self.b
+        return self.d.moe_mx_matmul(x, xs, rows, 1, off, w, ws, FP8, out, F32, None, len(self.x), n, 1, self.K, self.N)
+
+    def want(self, rows):
+        return (R.decode(self.x, self.xs, FP8) @ self.wd.T).astype(np.float32)[rows]
+
+
+def free_bytes():
+    import torch
+
+    return torch.cuda.mem_get_info()[0]
+
+
+def test_workspace_of_growing_batches_is_bounded(ds3, B):
+    """Batches that grow step by step: what the library keeps stays within a
+    small multiple of the largest, not the sum of them all."""
+    ds3.shutdown()
+    assert ds3.init() == 0
+    s = Sorted(ds3, B, 1)
+    sizes = range(16000, 40001, 500)
+    rows = I.rng(3).integers(0, 64, sizes[-1]).astype(np.int32)
+    rb, ob = B.up(rows), B.up(np.zeros((sizes[-1], s.N), np.float32))
+    offs = [B.up(np.array([0, n], np.int32)) for n in sizes]
+    assert s.call(ob, rb, offs[0], sizes[0]) == 0  # kernels loaded, a first block
+    before, scratch = free_bytes(), sizes[-1] * s.K * 33 // 32
+    for n, off in zip(sizes, offs):
+        assert s.call(ob, rb, off, n) == 0, ds3.last_error()
+    held = before - free_bytes()
+    assert_bitexact(B.down(ob, np.float32, (sizes[-1], s.N)), s.want(rows), "the largest batch")
+    assert held <= 2 * scratch, f"{held >> 20} MB kept for batches of at most {scratch >> 20} MB"
+
+
+@pytest.mark.parametrize("capture", ["graph_begin", "the host's"])
+def test_workspace_growth_between_a_capture_and_its_replay(ds3, B, capture):
+    """A captured product keeps the block that it sorts into when larger calls
+    outgrow it, whoever captures the module stream; the blocks that nothing
+    captured go back, inside a batch too."""
+    import torch
+
+    ds3.shutdown()
+    assert ds3.init() == 0
+    s = Sorted(ds3, B, 5)
+    n = 3000
+    rows = [I.rng(7 + i).integers(0, 64, 30 * n).astype(np.int32) for i in range(3)]
+    rb = [B.up(r) for r in rows]
+    out, big = B.up(np.zeros((n, s.N), np.float32)), B.up(np.zeros((30 * n, s.N), np.float32))
+    off = B.up(np.array([0, n], np.int32))
+    assert s.call(out, rb[0], off, n) == 0
+    stream = torch.cuda.ExternalStream(ds3.stream())
+    if capture == "graph_begin":
+        assert ds3.graph_begin() == 0
+        rc = s.call(out, rb[0], off, n)
+        g = ds3.graph_end()
+        replay, free = lambda: ds3.graph_launch(g), lambda: ds3.graph_free(g)  # noqa: E731
+    else:
+        assert ds3.begin_batch() == 0
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream, capture_error_mode="thread_local"):
+            rc = s.call(out, rb[0], off, n)
+        assert ds3.end_batch() == 0, ds3.last_error()
+
+        def replay():
+            with torch.cuda.stream(stream):
+                g.replay()
+            return 0
+
+        free = g.reset
+    assert rc == 0, ds3.last_error()
+    try:
+        for step, m in enumerate((4, 10, 30)):
+            boff = B.up(np.array([0, m * n], np.int32))
+            assert ds3.begin_batch() == 0
+            assert s.call(big, rb[1], boff, m * n) == 0
+            assert replay() == 0
+            assert s.call(big, rb[2], boff, m * n) == 0
+            assert ds3.end_batch() == 0, ds3.last_error()
+            assert_bitexact(B.down(out, np.float32, (n, s.N)), s.want(rows[0][:n]), f"replay {step}")
+            assert_bitexact(B.down(big, np.float32, (30 * n, s.N))[: m * n], s.want(rows[2][: m * n]), f"batch {step}")
+            rows[0] = I.rng(40 + step).integers(0, 64, 30 * n).astype(np.int32)
+            assert ds3.buffer_write(rb[0], 0, rows[0]) == 0
+    finally:
+        free()
+
+
+def test_workspace_that_does_not_fit(ds3, B):
+    """Scratch for more rows than the device holds: the call succeeds without
+    it, again and again, and smaller calls still get theirs. (The one group has
+    no rows, so nothing is read or written.)"""
+    s = Sorted(ds3, B, 9)
+    n = 1 << 27  # 258 GiB of sorted rows
+    rb, ob = ds3.empty(4 * n), ds3.empty(4 * n * 1)
+    B.all += [rb, ob]
+    none = B.up(np.zeros(2, np.int32))
+    x, xs, w, ws = s.b
+    for _ in range(3):
+        assert ds3.moe_mx_matmul(x, xs, rb, 1, none, w, ws, FP8, ob, F32, None, 64, n, 1, s.K, 1) == 0, ds3.last_error()
+    rows = I.rng(3).integers(0, 64, 500).astype(np.int32)
+    out = B.up(np.zeros((500, s.N), np.float32))
+    assert s.call(out, B.up(rows), B.up(np.array([0, 500], np.int32)), 500) == 0
+    assert_bitexact(B.down(out, np.float32, (500, s.N)), s.want(rows), "out")
