@@ -207,18 +207,25 @@ def prepare(case, seed):
     return s
 
 
-_ds3 = None
+_ds3 = _stream = None
 
 
 def _handles(s):
-    """The library's handles of the state's tensors; the first call opens the library and the batch that ops queue in."""
-    global _ds3
+    """The library's handles of the state's tensors; the first call opens the library and the batch that ops queue in.
+
+    Ops run on the library's own stream, which is not ordered with torch's: here it is put behind the inputs that
+    torch is still making, and a program that reads the outputs waits for the device (or lets its stream wait for the
+    library's) once behind its last op. What ops report on the device is read here too, behind those of earlier states."""
+    global _ds3, _stream
     if _ds3 is None:
         from qw3_b200 import ds3
 
         if ds3.init() != 0 or ds3.begin_batch() != 0:
             raise RuntimeError(ds3.last_error())
-        _ds3 = ds3
+        _ds3, _stream = ds3, torch.cuda.ExternalStream(ds3.stream())
+    if _ds3.device_errors() != 0:
+        raise RuntimeError("an op on an earlier state reported an error on the device")
+    _stream.wait_stream(torch.cuda.current_stream())
     return {k: _ds3.buffer_wrap(t.data_ptr(), t.numel() * t.element_size())
             for k, t in s.items() if isinstance(t, torch.Tensor)}
 
