@@ -188,6 +188,19 @@ def test_norm_optional_outputs(ds3, B):
     check_norm(x, x, w, 1e-5, run_norm(ds3, B, x, x, w, eps=1e-5, norm_out=False, sum_out=False))
 
 
+@pytest.mark.parametrize("rows,n", [(1000, 5120), (700, 8192), (1500, 8224), (470, 16384)])
+@pytest.mark.parametrize("form", ["plain", "no residual", "x", "r", "norm"])
+def test_norm_long_rows_many_per_warp(ds3, B, rows, n, form):
+    """Rows staged in shared memory, two and more to each warp, so that every
+    slot is used again: two slots up to 8192 elements, one past that. (Rows
+    without a residual take half the space, and twice the warps fit.)"""
+    rows *= 2 if form == "no residual" else 1
+    x, r, w = I.normal(rows, (rows, n)), I.normal(rows + 1, (rows, n), 0.0, 2.0), I.gamma(n, 3)
+    r = None if form == "no residual" else r
+    alias = form if form in ("x", "r", "norm") else None
+    check_norm(x, r, w, 1e-6, run_norm(ds3, B, x, r, w, alias=alias))
+
+
 def test_norm_extreme_rows(ds3, B):
     """Zero rows, rows whose squares pass fp32's range either way."""
     x, w = I.normal(1, (6, 128)), I.gamma(128, 3)
@@ -630,6 +643,64 @@ def test_swiglu(ds3, B, rows, E, K, F, fmt, mapped):
     check_act(got_q[:rows], got_s[:rows], h, slack)
 
 
+@pytest.mark.parametrize("rows,E", [(3000, 40), (3000, 14)])
+@pytest.mark.parametrize("fmt", [FP8, FP4])
+@pytest.mark.parametrize("mapped", [False, True])
+def test_swiglu_many_tiles_per_cta(ds3, B, rows, E, fmt, mapped):
+    """Several tiles for every CTA at the wide token blocks: accumulators,
+    column tables, exchange buffers and weights looked up ahead pass from tile
+    to tile."""
+    K, F, used = 256, 1504, 4
+    n_x = rows // 2
+    x, xs = R.encode(I.normal(1, (rows if not mapped else n_x, K)), FP8)
+    w = [R.encode(I.normal(i, (E, F, K), 0.0, K**-0.5), fmt) for i in (2, 3)]
+    off, g = ragged(4, rows, E, 0.1), I.rng(5)
+    x_rows = g.integers(0, n_x * used, rows).astype(np.int32) if mapped else None
+    rw = g.random(n_x * used if mapped else rows).astype(np.float32) + np.float32(0.1)
+    q, s = B.up(np.full((rows, F), 0x33, np.uint8)), B.up(np.full((rows, F // 32), 0x33, np.uint8))
+    assert ds3.moe_mx_swiglu(B.up(x), B.up(xs), B.up(x_rows), used, B.up(off), B.up(w[0][0]), B.up(w[0][1]), B.up(w[1][0]),
+                             B.up(w[1][1]), fmt, B.up(rw), q, s, len(x), rows, E, K, F) == 0, ds3.last_error()
+    src = x_rows // used if mapped else np.arange(rows)
+    h, slack = exact_act(R.decode(x, xs, FP8), [R.decode(*p, fmt) for p in w], off, src,
+                         rw[x_rows if mapped else np.arange(rows)].astype(np.float64))
+    check_act(B.down(q, np.uint8, (rows, F)), B.down(s, np.uint8, (rows, F // 32)), h, slack)
+
+
+@pytest.mark.parametrize("rows,E", [(3000, 40), (3000, 14)])
+@pytest.mark.parametrize("fmt", [FP8, FP4])
+def test_swiglu_gathers_where_the_workspace_cannot_grow(ds3, B, rows, E, fmt):
+    """A capture before any workspace exists: every width gathers its rows in
+    the kernel. Outside, the same call sorts them first where the groups are
+    large; both give the same codes."""
+    ds3.shutdown()
+    assert ds3.init() == 0
+    K, F, used = 256, 736, 2
+    n_x = rows // 2
+    x, xs = R.encode(I.normal(1, (n_x, K)), FP8)
+    w = [R.encode(I.normal(i, (E, F, K), 0.0, K**-0.5), fmt) for i in (2, 3)]
+    off, g = ragged(4, rows, E, 0.1), I.rng(5)
+    x_rows = g.integers(0, n_x * used, rows).astype(np.int32)
+    rw = g.random(n_x * used).astype(np.float32) + np.float32(0.1)
+    b = [B.up(v) for v in (x, xs, x_rows, off, *w[0], *w[1], rw)]
+    outs = [(B.up(np.zeros((rows, F), np.uint8)), B.up(np.zeros((rows, F // 32), np.uint8))) for _ in range(2)]
+    call = lambda o: ds3.moe_mx_swiglu(b[0], b[1], b[2], used, *b[3:8], fmt, b[8], *o, n_x, rows, E, K, F)  # noqa: E731
+    assert ds3.graph_begin() == 0
+    rc = call(outs[0])
+    g = ds3.graph_end()
+    assert rc == 0, ds3.last_error()
+    for _ in range(2):
+        assert ds3.graph_launch(g) == 0
+    ds3.synchronize()
+    ds3.graph_free(g)
+    assert call(outs[1]) == 0
+    got = [(B.down(q, np.uint8, (rows, F)), B.down(s, np.uint8, (rows, F // 32))) for q, s in outs]
+    assert_bitexact(got[0][0], got[1][0], "gathered and sorted elements")
+    assert_bitexact(got[0][1], got[1][1], "gathered and sorted scales")
+    h, slack = exact_act(R.decode(x, xs, FP8), [R.decode(*p, fmt) for p in w], off, x_rows // used,
+                         rw[x_rows].astype(np.float64))
+    check_act(*got[0], h, slack)
+
+
 def test_swiglu_bad_rows_and_large_gates(ds3, B):
     """A row id outside x gives zeros; gates far from zero saturate silu to
     0 and the identity without NaN."""
@@ -789,6 +860,86 @@ def test_layer_graph_replay_on_new_inputs(ds3, B, fmt):
             for layer, e in zip(layers, eager):
                 for k, v in layer.outputs().items():
                     assert_bitexact(v, e[k], k)
+    finally:
+        ds3.graph_free(g)
+
+
+@pytest.mark.parametrize("fmt", [FP8, FP4])
+def test_layers_that_sort_in_one_batch_and_in_a_graph(ds3, B, fmt):
+    """Groups large enough for the row sort: two layers in one batch write the
+    same workspace behind one another; captured, they replay on new inputs,
+    also after a larger call has outgrown the block they were captured with."""
+    layers = [Layer(ds3, B, 700, fmt, seed=50), Layer(ds3, B, 700, fmt, seed=80)]
+    assert ds3.begin_batch() == 0
+    for layer in layers:
+        layer.enqueue()
+    assert ds3.end_batch() == 0, ds3.last_error()
+    for layer in layers:
+        layer.check(layer.outputs())
+    assert ds3.graph_begin() == 0
+    for layer in layers:
+        layer.enqueue()
+    g = ds3.graph_end()
+    try:
+        for step in range(3):
+            if step == 2:
+                Layer(ds3, B, 9000, fmt, seed=20).enqueue()
+            for i, layer in enumerate(layers):
+                layer.lg = I.normal(200 + 10 * step + i, layer.lg.shape, 0.0, 1.0 + 3 * step)
+                layer.x = I.normal(300 + 10 * step + i, layer.x.shape)
+                assert ds3.buffer_write(layer.b["lg"], 0, layer.lg) == 0
+                assert ds3.buffer_write(layer.b["x"], 0, layer.x) == 0
+            for _ in range(2):
+                assert ds3.graph_launch(g) == 0
+            ds3.synchronize()
+            for layer in layers:
+                layer.check(layer.outputs())
+    finally:
+        ds3.graph_free(g)
+
+
+@pytest.mark.parametrize("T,E,K", [(37, 16, 4), (8200, 40, 8)])
+def test_rows_captured_and_combined_through_the_inverse_map(ds3, B, T, E, K):
+    """moe_expert_rows in a graph, at both of its forms, replayed on other ids;
+    row_of takes the sorted product's rows back to their tokens in
+    moe_combine_residual, as out_rows = entries does in the product."""
+    H, F = 64, 32
+    a, as_ = exact_rows(1, T * K, F, FP8)
+    w, ws = exact_rows(2, E * H, F, FP8)
+    ad, wd = R.decode(a, as_, FP8), R.decode(w, ws, FP8).reshape(E, H, F)
+    n, z = T * K, lambda *s: B.up(np.zeros(s, np.int32))  # noqa: E731
+    sc, res = I.rng(3).random((T, K)).astype(np.float32), I.normal(4, (T, H))
+    idx, off, ent, row, y, out, y2, out2 = z(n), z(E + 1), z(n), z(n), z(n, H), z(T, H), z(n, H), z(T, H)
+    b = [B.up(v) for v in (a, as_, w, ws, sc, res)]
+
+    def enqueue():
+        assert ds3.moe_expert_rows(idx, off, ent, row, T, E, K) == 0
+        for dst, to, back, o in ((y, None, row, out), (y2, ent, None, out2)):
+            assert ds3.moe_mx_matmul(b[0], b[1], None, 1, off, b[2], b[3], FP8, dst, F32, to, n, n, E, F, H) == 0
+            assert ds3.moe_combine_residual(dst, back, b[4], b[5], o, T, K, H) == 0
+
+    ids = [np.argsort(I.rng(7 + i).random((T, E)), 1)[:, :K].astype(np.int32) for i in range(3)]
+    assert ds3.buffer_write(idx, 0, ids[0]) == 0
+    enqueue()
+    assert ds3.graph_begin() == 0
+    enqueue()
+    g = ds3.graph_end()
+    try:
+        for i in ids[1:]:
+            assert ds3.buffer_write(idx, 0, i) == 0
+            assert ds3.graph_launch(g) == 0
+            ds3.synchronize()
+            want = R.expert_rows(i, E)
+            for got, v in zip((B.down(v, np.int32, (k,)) for v, k in ((off, E + 1), (ent, n), (row, n))), want):
+                assert_bitexact(got, v)
+            ys = R.grouped(ad, wd, want[0], np.arange(n)).astype(np.float32)
+            assert_bitexact(B.down(y, np.float32, (n, H)), ys, "sorted rows")
+            total = B.down(out, np.float32, (T, H))
+            assert_bitexact(total, B.down(out2, np.float32, (T, H)), "row_of and entries")
+            terms = ys[want[2]].reshape(T, K, H).astype(np.float64) * sc[:, :, None]
+            # K products and K + 1 sums, half a step each
+            tol = (2 * K + 1) * 2.0**-24 * (np.abs(terms).sum(1) + np.abs(res))
+            assert (np.abs(total - (res + terms.sum(1))) <= tol).all()
     finally:
         ds3.graph_free(g)
 
