@@ -944,6 +944,39 @@ def test_rows_captured_and_combined_through_the_inverse_map(ds3, B, T, E, K):
         ds3.graph_free(g)
 
 
+@pytest.mark.parametrize("fmt", [FP8, FP4])
+def test_weights_converted_expert_by_expert(ds3, B, fmt):
+    """Q8_0 expert tensors to MX weights through one expert's fp32 scratch, in
+    one batch, and into a product."""
+    E, N, K, rows = 5, 96, 256, 40
+    g = I.rng(8)
+    d = g.uniform(0.001, 0.01, (E, N, K // 32, 1)).astype(np.float16)
+    codes = g.integers(-127, 128, (E, N, K // 32, 32)).astype(np.int8)
+    src = B.up(np.concatenate([d.view(np.uint8), codes.view(np.uint8)], -1))
+    w = (d.astype(np.float32) * codes.astype(np.float32)).reshape(E, N, K)
+    per = N * K // (2 if fmt == FP4 else 1)
+    tmp, q, s = (B.up(np.zeros(v, np.uint8)) for v in (N * K * 4, E * per, E * N * K // 32))
+
+    def view(b, i, n):
+        B.all.append(ds3.buffer_view(b, i * n, n))
+        return B.all[-1]
+
+    assert ds3.begin_batch() == 0
+    for e in range(E):
+        assert ds3.dequantize_f32(view(src, e, N * K // 32 * 34), 8, N * K, tmp) == 0, ds3.last_error()
+        assert ds3.mx_quantize(tmp, F32, view(q, e, per), view(s, e, N * K // 32), fmt, N, K) == 0, ds3.last_error()
+    assert ds3.end_batch() == 0, ds3.last_error()
+    wq, ws = R.encode(w, fmt)
+    assert_bitexact(B.down(q, np.uint8, wq.shape), wq, "elements")
+    assert_bitexact(B.down(s, np.uint8, ws.shape), ws, "scales")
+    x, xs = R.encode(I.normal(1, (rows, K)), FP8)
+    off, out = ragged(3, rows, E), B.up(np.zeros((rows, N), np.float32))
+    assert ds3.moe_mx_matmul(B.up(x), B.up(xs), None, 1, B.up(off), q, s, fmt, out, F32, None, rows, rows, E, K, N) == 0
+    xd, wd = R.decode(x, xs, FP8), R.decode(wq, ws, fmt)
+    want, size = (R.grouped(a, b, off, np.arange(rows)) for a, b in ((xd, wd), (np.abs(xd), np.abs(wd))))
+    assert (np.abs(B.down(out, np.float32, (rows, N)) - want) <= K * 2.0**-23 * size).all()
+
+
 # ------------------------------------------------------------- the workspace
 class Sorted:
     """A product over mapped rows that are sorted into the workspace first, with exact operands."""
