@@ -30,10 +30,10 @@
 //     scaling are exact; the only roundings are the fp32 accumulation's.
 //   - MXFP4 weights are expanded to one byte per element by the copy engine
 //     (packed in HBM, 16 elements per 16 bytes in shared memory).
-//   - SwiGLU's A tile is 64 gate rows over the same 64 up rows, so the four
-//     epilogue warps (one per 32 tensor-memory lanes) pair up: gate and up meet
-//     through a shared-memory exchange, and a warp's 32 lanes of a column are
-//     the 32 elements of one MX block.
+//   - SwiGLU's A tile is 64 gate rows over the same 64 up rows. Two sides of four
+//     epilogue warps (one per 32 tensor-memory lanes) take alternate chunks of 16
+//     columns; a side's warps pair up, gate and up meet through a shared-memory
+//     exchange, and eight lanes with four elements each finish one MX block.
 //
 // Warps: 0 copies (weights, and token rows that are used in place, as tiled
 // boxes), 1 issues the tensor-core work, 2 / 3 stage the scales of A / B in the
@@ -44,8 +44,9 @@
 // expert the weights' HBM bytes: 512 tokens x top-8 of 128 experts, 2048 -> 2 x
 // 768: MXFP8 5.6 TB/s. MXFP4 halves the bytes, and then the issuing warp's and
 // the copy engine's work per stage bounds it (4.3 TB/s). Long batches: the
-// operands' way from L2 to the SMs (about 10 TB/s there) and power: 4096
-// tokens, 1.35 PFLOP/s in place. The epilogue then counts too (20 of 150 us).
+// operands' way from L2 to the SMs (12.7 TB/s there) and power: 4096 tokens in
+// place 148 us after a pause (1.39 PFLOP/s), 178 us in calls back to back; the
+// row sort before it is 19 us more. The epilogue counts too (20 of 150 us).
 //
 // Every wait is bounded; on a timeout the CTA records it, lets its copies and
 // products land (bounded), frees its tensor memory and returns.
@@ -969,10 +970,15 @@ static int moe_mean_rows(int n_rows, int n_group) { return (n_rows + n_group - 1
 
 // Gathering inside the product kernel goes through the threads' copy path,
 // which cannot feed wide tiles; sorting the rows first costs a pass over them.
-// Measured, 128 groups, 2048 -> 2 x 768, us gathered / sorted first: MXFP8
-// weights, mean 32 rows 74 / 79, 64: 80 / 85, 80: 83 / 90, 96: 90 / 93, 112:
-// 97 / 95, 128: 118 / 107; MXFP4, whose weights hide less of it, 32: 50 / 53,
-// 64: 67 / 65, 80: 74 / 70, 96: 82 / 72, 128: 118 / 91.
+// Measured, 128 groups of random sizes, us gathered / sorted first, SwiGLU 2048
+// -> 2 x 768 and (fp16) 768 -> 2048:
+//   mean rows     32         48         64         80          96          128
+//   MXFP8 SwiGLU  73 / 78    77 / 83    83 / 87    92 / 93     100 / 97    131 / 115
+//         plain   41 / 43    44 / 45    49 / 47    52 / 51     56 / 54     73 / 63
+//   MXFP4 SwiGLU  53 / 56    63 / 63    72 / 71    81 / 77     90 / 83     120 / 103
+//         plain   32 / 33    36 / 36    42 / 39    46 / 44     50 / 47     66 / 58
+// The limits are SwiGLU's, where token rows are gathered; a plain product over
+// x_rows would gain 2 to 4 % from 64 rows of MXFP8 on.
 size_t moe_sort_bytes(const MoeMxCall &q)
 {
     if (!q.x_rows || moe_mean_rows(q.n_rows, q.n_group) <= (q.w_type == kMxFp4 ? 48 : 96)) return 0;
@@ -1025,11 +1031,19 @@ cudaError_t launch_moe_mx(const LaunchCtx &c, const MoeMxCall &q)
         !encode(&maps.w1, swiglu ? q.w1 : q.w0, 3, q.K, q.n_w, q.n_group, kTileM / 2, fp4) ||
         !encode(&maps.x, a.x, 2, q.K, n_map, 1, 32, false))
         return cudaErrorInvalidValue;
-    // Token columns per tile by the groups' mean size. Measured over 128 groups,
-    // 2048 -> 2 x 768, MXFP8, us at 64 / 128 / 224 columns: mean 32: 71 / 73 /
-    // 80, 48: 74 / 74 / 82, 64: 80 / 76 / 84, 96: 100 / 82 / 89, 128: 119 / 99 /
-    // 96, 256: 200 / 157 / 158. (Half of the groups of about 128 rows need a
-    // second block of 128.)
+    // Token columns per tile by the groups' mean size. Measured over 128 groups of
+    // random sizes, rows in place, us at 64 / 128 / 224 columns, SwiGLU 2048 -> 2 x
+    // 768 and (fp16) 768 -> 2048:
+    //   mean   MXFP8 SwiGLU     MXFP8 plain     MXFP4 SwiGLU     MXFP4 plain
+    //   48     74 / 76 / 84     41 / 40 / 44    56 / 59 / 70     32 / 32 / 38
+    //   64     87 / 80 / 88     47 / 43 / 47    74 / 65 / 74     40 / 35 / 41
+    //   112    117 / 91 / 100   63 / 51 / 54    104 / 80 / 87    56 / 44 / 48
+    //   128    134 / 109 / 105  71 / 59 / 57    120 / 98 / 93    64 / 53 / 51
+    //   192    181 / 145 / 126  97 / 79 / 69    164 / 131 / 116  88 / 72 / 63
+    //   256    232 / 175 / 178  123 / 98 / 98   211 / 163 / 166  114 / 91 / 92
+    //   512    419 / 308 / 301  224 / 176 / 164 389 / 292 / 286  210 / 168 / 157
+    // (Half of the groups of about 128 rows need a second block of 128; groups of
+    // about 256 take two blocks of 224, and two or three of 128.)
     const int avg = moe_mean_rows(q.n_rows, q.n_group);
     const int nt = avg <= 48 ? 64 : avg <= 112 ? 128 : 224;
 #define DS3_MOE(NT)                                                                                                  \

@@ -136,7 +136,8 @@ __global__ void __launch_bounds__(256) mx_dequantize_k(const uint8_t *q, const u
 // 16384 x 2048: 93 us, 6.2 TB/s; without the prefetch of the next wave's rows
 // 103 us; with one warp per row and the row in shared memory, the first
 // version, 149 us (too few reads in flight behind its chains).
-// Longer rows: that version, below.
+// Longer rows: that version, below (2048 x 8192 with residual and every output:
+// 274 us, 1.0 TB/s; 4096 x 5120: 206 us, 1.7 TB/s).
 constexpr int kNormMxMaxN = 16384;
 
 // 1 / sqrt(m) to full fp64 accuracy: the fp32 estimate and two Newton steps,
@@ -192,8 +193,9 @@ __device__ __forceinline__ double sumsq4(float4 v, double acc)
     return fma((double)v.w, (double)v.w, acc);
 }
 
-// FEW: one wave of rows at most. Registers are free then, and the norm weight
-// (a parameter the operation just before must not write) is loaded before the
+// FEW: at most 8 rows per SM, one wave of short rows and up to three of the
+// longest. Registers are free then (40 to 162 a thread), and the norm weight (a
+// parameter the operation just before must not write) is loaded before the
 // programmatic-launch wait, which takes a round trip out of the chain.
 template <int VPT, bool FEW>
 __global__ void __launch_bounds__(128, FEW ? 1 : VPT <= 4 ? 8 : 4) add_rms_norm_mx_row(const float *x, const float *r, const float *w, float *sum_out,
@@ -202,8 +204,8 @@ __global__ void __launch_bounds__(128, FEW ? 1 : VPT <= 4 ? 8 : 4) add_rms_norm_
     __shared__ double part[4];
     const int tid = threadIdx.x, n4 = n / 4;
     const int64_t row = blockIdx.x;
-    // Into L2: a first row while the previous kernel runs, later on the row that
-    // a CTA of the next wave will read.
+    // Into L2: a first row while the previous kernel runs, later on the row `ahead`
+    // behind this one.
     auto prefetch = [&](int64_t at) {
         const float *p = tid ? r : x;
         if (tid < 2 && p) prefetch_l2(p + at * n, (uint64_t)n * 4);
@@ -433,7 +435,9 @@ cudaError_t launch_add_rms_norm_mx(const LaunchCtx &c, const float *x, const flo
     if (n <= 4096) {
         if (rows > 0x7fffffffLL) return cudaErrorInvalidValue;
         const dim3 g((unsigned)rows), b(128);
-        const int ahead = c.n_sm * 8;  // about one wave of rows
+        // About one wave of rows up to 2048 elements (8 CTAs per SM, more of the
+        // shortest), two waves of longer ones (4 per SM).
+        const int ahead = c.n_sm * 8;
         const double inv_n = 1.0 / n;
 #define DS3_NORM(VPT)                                                                                                  \
     (rows <= ahead ? launch_k(c, add_rms_norm_mx_row<VPT, true>, g, b, x, r, w, sum_out, norm_out, q, scales, n, inv_n, \
